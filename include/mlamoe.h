@@ -329,6 +329,33 @@ MM_API int mm_lm_head_dev(mm_ctx *ctx, int B, const float *x, const uint16_t *no
                           const uint16_t *lm_head, int vocab, int hidden, float *logits,
                           int32_t *tokens);
 
+/* Log probabilities, entropies and top alternatives of T rows of logits: what
+ * ranks and reports sampled tokens, or scores given ones.  No counterpart in
+ * the reference, which samples greedily (src/run.c:503-508).  Row t is the n
+ * floats at logits + t * stride (stride in floats, >= n; mm_lm_head_dev and
+ * the engine's steps write stride = n), targets [T] token indices.  Any output
+ * may be NULL:
+ *   logprob [T]             log softmax(row)[targets[t]] (targets may be NULL
+ *                           with logprob); -inf for a logit of -inf, NaN for a
+ *                           target outside [0, n)
+ *   entropy [T]             -sum p log p, in nats
+ *   top_idx, top_logprob    [T, n_top] the n_top largest logits' tokens and log
+ *                           probabilities, descending, of equal ones (-0 and 0
+ *                           too) the lowest token first
+ * n_top <= 32 and <= n; n <= 2^30.  A row's -inf logits are tokens of
+ * probability 0, listed after every other.  NaN logits are never listed: with
+ * fewer than n_top numbers in a row the rest is -1 and NaN.  A row that holds a
+ * NaN or +inf, or nothing above -inf, has no distribution: its logprob, entropy
+ * and top_logprob are NaN, its top_idx as ever.  Inputs are not changed.
+ * Device pointers, asynchronous.  Workspace: `ws`, ws_bytes >=
+ * mm_token_logprobs_workspace of it, 16-byte aligned, device memory of the
+ * caller's that no other call uses until this one is done (needed under stream
+ * capture); or NULL: the context's. */
+MM_API int mm_token_logprobs_dev(mm_ctx *ctx, int T, const float *logits, size_t stride, int n,
+                                 const int32_t *targets, float *logprob, float *entropy, int n_top,
+                                 int32_t *top_idx, float *top_logprob, void *ws, size_t ws_bytes);
+MM_API int mm_token_logprobs_workspace(int T, int n, int n_top, size_t *bytes);
+
 /* ---- MLA absorbed decode --------------------------------------------------- */
 
 /* The attention fields of the reference Config (include/model.h:12-42). */

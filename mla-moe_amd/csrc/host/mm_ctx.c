@@ -102,6 +102,9 @@ static const struct {
     [K_F32_BF16] = {"mm_f32_bf16", MOD_UTIL},
     [K_ROUTER_WIDE] = {"mm_router_wide", MOD_MOE_BF16},
     [K_ROUTE_WIDE] = {"mm_route_wide", MOD_MOE_I8},
+    [K_LOGPROBS] = {"mm_logprobs", MOD_LM_HEAD},
+    [K_LOGPROBS_1] = {"mm_logprobs_1", MOD_LM_HEAD},
+    [K_LOGPROBS_FINAL] = {"mm_logprobs_final", MOD_LM_HEAD},
 };
 
 /* ---- errors ------------------------------------------------------------- */
@@ -413,6 +416,21 @@ int mm_workspace(mm_ctx *c, size_t bytes, void **out) {
     }
     *out = c->ws;
     return MM_OK;
+}
+
+int mm_call_workspace(mm_ctx *c, const char *name, void *ws, size_t ws_bytes, size_t need, void **out) {
+    if (ws) {
+        if ((uintptr_t)ws % 16) return mm_fail(MM_ERR_INVALID, "%s: workspace must be 16-byte aligned", name);
+        if (ws_bytes < need)
+            return mm_fail(MM_ERR_INVALID, "%s: workspace of %zu bytes, %zu needed", name, ws_bytes, need);
+        *out = ws;
+        return MM_OK;
+    }
+    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+    MM_HIP(hipStreamIsCapturing(c->stream, &cs));
+    if (cs != hipStreamCaptureStatusNone)
+        return mm_fail(MM_ERR_STATE, "%s: a captured call needs a workspace of its own", name);
+    return mm_workspace(c, need, out);
 }
 
 int mm_io_buffer(mm_ctx *c, size_t bytes, void **out) {

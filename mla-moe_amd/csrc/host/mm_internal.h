@@ -79,6 +79,9 @@ typedef enum {
     K_F32_BF16,
     K_ROUTER_WIDE,
     K_ROUTE_WIDE,
+    K_LOGPROBS,
+    K_LOGPROBS_1,
+    K_LOGPROBS_FINAL,
     K_COUNT
 } mm_kernel_id;
 
@@ -207,6 +210,10 @@ int mm_launch(mm_ctx *ctx, mm_kernel_id id, unsigned gx, unsigned gy, unsigned g
 /* Device workspace of at least `bytes`, reallocated (after a stream sync)
  * when too small. */
 int mm_workspace(mm_ctx *ctx, size_t bytes, void **out);
+/* The workspace of a call that takes the caller's (`ws` of `ws_bytes`, 16-byte
+ * aligned) or, with ws NULL, the context's: `need` bytes.  Not the context's
+ * while its stream is captured, since a later call may move it. */
+int mm_call_workspace(mm_ctx *ctx, const char *name, void *ws, size_t ws_bytes, size_t need, void **out);
 /* Device staging of at least `bytes` for the host-pointer entry points (a
  * buffer of its own: the forward calls they make use the workspace). */
 int mm_io_buffer(mm_ctx *ctx, size_t bytes, void **out);

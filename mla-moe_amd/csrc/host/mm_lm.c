@@ -1,5 +1,6 @@
 /* mm_lm.c -- the decode step's LM head (host side): final RMSNorm, logits
- * over the vocabulary, greedy argmax (src/run.c:22-27, 493-494, 503-508). */
+ * over the vocabulary, greedy argmax (src/run.c:22-27, 493-494, 503-508),
+ * log probabilities of tokens. */
 #include "mm_internal.h"
 
 static size_t al256(size_t b) { return (b + 255) & ~(size_t)255; }
@@ -38,6 +39,65 @@ int mm_argmax_dev(mm_ctx *c, int T, const float *logits, int n, int32_t *tokens)
     char *ws;
     if ((st = mm_workspace(c, argmax_ws(T, n), (void **)&ws))) return st;
     return argmax_launch(c, T, logits, n, tokens, ws);
+}
+
+/* Elements per segment and segments per row: rows are cut until the grid has
+ * MM_LP_BLOCKS blocks (four per CU), in whole passes of a block. */
+static int logprobs_seg(int T, int n, int *nseg) {
+    const int passes = (n + MM_LP_PASS - 1) / MM_LP_PASS;
+    int s = (MM_LP_BLOCKS + T - 1) / T;
+    if (s > passes) s = passes;
+    if (s > MM_LP_SEG_MAX) s = MM_LP_SEG_MAX;
+    const int pp = (passes + s - 1) / s;
+    *nseg = (passes + pp - 1) / pp;
+    return pp * MM_LP_PASS;
+}
+
+static int logprobs_check(int T, int n, int n_top) {
+    if (T < 0 || n <= 0 || n_top < 0 || n_top > n)
+        return mm_fail(MM_ERR_INVALID, "mm_token_logprobs: bad shape");
+    if (n_top > MM_LP_TOP_MAX || n > 1 << 30)
+        return mm_fail(MM_ERR_UNSUPPORTED, "mm_token_logprobs: n_top <= %d, n <= 2^30", MM_LP_TOP_MAX);
+    return MM_OK;
+}
+
+int mm_token_logprobs_workspace(int T, int n, int n_top, size_t *bytes) {
+    if (!bytes) return mm_fail(MM_ERR_INVALID, "mm_token_logprobs_workspace: NULL argument");
+    *bytes = 0;
+    int st = logprobs_check(T, n, n_top), nseg;
+    if (st || T == 0) return st;
+    logprobs_seg(T, n, &nseg);
+    if (nseg > 1) *bytes = al256((size_t)T * nseg * 16) + 2 * al256((size_t)T * nseg * n_top * 4);
+    return MM_OK;
+}
+
+int mm_token_logprobs_dev(mm_ctx *c, int T, const float *logits, size_t stride, int n,
+                          const int32_t *targets, float *logprob, float *entropy, int n_top,
+                          int32_t *top_idx, float *top_logprob, void *ws, size_t ws_bytes) {
+    if (!c || (T > 0 && !logits) || (T > 0 && logprob && !targets))
+        return mm_fail(MM_ERR_INVALID, "mm_token_logprobs_dev: NULL argument");
+    int st = logprobs_check(T, n, n_top), nseg;
+    if (st) return st;
+    if (T > 1 && stride < (size_t)n)
+        return mm_fail(MM_ERR_INVALID, "mm_token_logprobs_dev: stride %zu < n %d", stride, n);
+    if ((uintptr_t)logits % 4) return mm_fail(MM_ERR_INVALID, "mm_token_logprobs_dev: logits must be 4-byte aligned");
+    if (!top_idx && !top_logprob) n_top = 0;
+    if (T == 0 || (!logprob && !entropy && n_top == 0)) return MM_OK;
+    if ((st = mm_set_device(c))) return st;
+    const int seg = logprobs_seg(T, n, &nseg);
+    if ((size_t)T * nseg > 0x7fffffffu)
+        return mm_fail(MM_ERR_UNSUPPORTED, "mm_token_logprobs_dev: %d rows of %d", T, n);
+    char *p = NULL;
+    const size_t n_s = al256((size_t)T * nseg * 16), n_v = al256((size_t)T * nseg * n_top * 4);
+    if (nseg > 1 &&
+        (st = mm_call_workspace(c, "mm_token_logprobs_dev", ws, ws_bytes, n_s + 2 * n_v, (void **)&p)))
+        return st;
+    mm_logprobs_args a = {logits, stride, targets, logprob, entropy, top_idx, top_logprob,
+                          (float *)p, (float *)(p + n_s), (int32_t *)(p + n_s + n_v), n, n_top, nseg, seg};
+    const int vec = (uintptr_t)logits % 16 == 0 && (T == 1 || stride % 4 == 0) && n >= 4;
+    if ((st = mm_launch(c, vec ? K_LOGPROBS : K_LOGPROBS_1, (unsigned)T * (unsigned)nseg, 1, 1, 256, 0, &a)))
+        return st;
+    return nseg > 1 ? mm_launch(c, K_LOGPROBS_FINAL, (unsigned)T, 1, 1, 64, 0, &a) : MM_OK;
 }
 
 int mm_lm_head_dev(mm_ctx *c, int B, const float *x, const uint16_t *norm, float eps,

@@ -700,6 +700,26 @@ typedef struct {
     int n, T, nseg;
 } mm_argmax_args;
 
+/* ---- log probabilities, entropies, top alternatives (logprobs.h) -------------- */
+#define MM_LP_TOP_MAX 32         /* alternatives per row at most */
+#define MM_LP_PASS 4096          /* elements of one pass of a block's four waves */
+#define MM_LP_SEG_MAX 64         /* segments per row at most */
+#define MM_LP_BLOCKS 1024        /* rows are cut into segments until the grid has this many blocks */
+typedef struct {
+    const float *logits;     /* [T, stride], the first n of a row used */
+    size_t stride;
+    const int32_t *targets;  /* [T], read where logprob is given */
+    float *logprob;          /* [T] or 0 */
+    float *entropy;          /* [T] or 0 */
+    int32_t *top_idx;        /* [T, n_top] or 0 */
+    float *top_logprob;      /* [T, n_top] or 0 */
+    float *part_s;           /* [T, nseg, 4]: m, R, U, list entries (as an int's bits) */
+    float *part_v;           /* [T, nseg, n_top] each segment's largest, sorted */
+    int32_t *part_i;         /* [T, nseg, n_top] their indices */
+    int n, n_top, nseg;
+    int seg;                 /* elements per segment, a multiple of MM_LP_PASS */
+} mm_logprobs_args;
+
 /* ---- dense GEMV for a few tokens (decode projections) ----------------------- */
 /* Up to two weight matrices ("segments") over one activation row set: rows
  * [0, rows0) of the row space are W0's, [rows0, rows0 + rows1) W1's;

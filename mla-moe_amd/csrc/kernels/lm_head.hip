@@ -21,6 +21,8 @@
  *   mm_argmax_part / mm_argmax_final   segments of every row in parallel
  *                (mm_lm_gemv and mm_lm_gemm write their partials themselves),
  *                then one block per row over the partials
+ *   mm_logprobs / mm_logprobs_final   log probabilities, entropies, top
+ *                alternatives (logprobs.h)
  */
 #include "gemv.h"
 
@@ -531,3 +533,5 @@ extern "C" __global__ __launch_bounds__(MM_LMG_THREADS, 1) void mm_lm_gemm(mm_lm
         a.part_i[(size_t)tid * gridDim.x + blockIdx.x] = ix;
     }
 }
+
+#include "logprobs.h"

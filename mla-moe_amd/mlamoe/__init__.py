@@ -152,6 +152,9 @@ def lib():
         L.mm_argmax_dev.argtypes = [_vp, C.c_int, _vp, C.c_int, _vp]
         L.mm_lm_head_dev.argtypes = [_vp, C.c_int, _vp, _vp, C.c_float, _vp, C.c_int, C.c_int,
                                      _vp, _vp]
+        L.mm_token_logprobs_dev.argtypes = [_vp, C.c_int, _vp, C.c_size_t, C.c_int, _vp, _vp, _vp, C.c_int,
+                                            _vp, _vp, _vp, C.c_size_t]
+        L.mm_token_logprobs_workspace.argtypes = [C.c_int, C.c_int, C.c_int, C.POINTER(C.c_size_t)]
         L.mm_moe_i8_layer_size.argtypes = [C.POINTER(MoeConfig), C.POINTER(C.c_size_t),
                                            C.POINTER(C.c_size_t)]
         L.mm_moe_export_layer_i8.argtypes = [_vp, C.c_int, _vp, _vp]
@@ -183,6 +186,13 @@ def rope_inv_freq(dim, theta, factor=1.0, beta_fast=32.0, beta_slow=1.0, orig_ma
     _check(lib().mm_rope_inv_freq(dim, theta, factor, beta_fast, beta_slow, orig_max,
                                   inv.ctypes.data_as(C.POINTER(C.c_float))))
     return inv
+
+
+def token_logprobs_workspace(T, n, n_top):
+    """Bytes of workspace of a token_logprobs_dev call."""
+    b = C.c_size_t()
+    _check(lib().mm_token_logprobs_workspace(T, n, n_top, C.byref(b)))
+    return b.value
 
 
 def _check(st):
@@ -542,6 +552,29 @@ class Context:
         tokens = dt.download()
         self._tmp((dx, dn, dw, dl, dt))
         return logits, tokens
+
+    def token_logprobs_dev(self, T, logits, stride, n, targets=None, logprob=None, entropy=None, n_top=0,
+                           top_idx=None, top_logprob=None, ws=None):
+        """mm_token_logprobs_dev over device buffers; ws: a DevBuf of
+        token_logprobs_workspace bytes, or None for the context's."""
+        p = lambda b: None if b is None else b.ptr  # noqa: E731
+        _check(lib().mm_token_logprobs_dev(self.h, T, p(logits), stride, n, p(targets), p(logprob), p(entropy),
+                                           n_top, p(top_idx), p(top_logprob), p(ws), ws.nbytes if ws is not None else 0))
+
+    def token_logprobs(self, logits, targets=None, n_top=0, n=None):
+        """Host arrays: logits [T, stride] fp32 (the first n of a row used),
+        targets [T].  Returns (logprob or None, entropy, top_idx, top_logprob)."""
+        lg = np.ascontiguousarray(logits, np.float32)
+        T, stride = lg.shape
+        n = stride if n is None else n
+        dl, de = self.to_device(lg), self.empty((T,), np.float32)
+        dt = self.to_device(np.ascontiguousarray(targets, np.int32)) if targets is not None else None
+        dp = self.empty((T,), np.float32) if targets is not None else None
+        di, dv = self.empty((T, n_top), np.int32), self.empty((T, n_top), np.float32)
+        self.token_logprobs_dev(T, dl, stride, n, dt, dp, de, n_top, di, dv)
+        out = dp.download() if dp is not None else None, de.download(), di.download(), dv.download()
+        self._tmp((dl, de, dt, dp, di, dv))
+        return out
 
     # MLA absorbed decode -------------------------------------------------------
     def mla_init(self, NH, QKN=128, QKR=64, KVL=512, VHD=128, scale=None, n_layers=1):
