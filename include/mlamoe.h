@@ -395,6 +395,51 @@ MM_API int mm_mla_absorbed_decode_dev(mm_ctx *ctx, int layer, int B, const float
                                       const int32_t *kv_lens, int kv_len, float *ctx_out,
                                       float *qabs, float *probs, float *clat);
 
+/* The absorbed decode for B sequences that continue one prefix, whose latent
+ * cache is held and read once for all of them (the reference keeps a whole
+ * cache per sequence, include/model.h:117): sequence b attends to the
+ * prefix_len rows of `prefix` and to the first kv_lens[b] rows of its own cache.
+ *   q        [B, NH, QKN + QKR] fp32, q_nope | q_pe (RoPE applied, at the
+ *            positions after the prefix; so is the own rows' k_pe)
+ *   prefix   [prefix_len, KVL + QKR] bf16, or NULL with prefix_len 0
+ *   cache    [B, seq_stride, KVL + QKR] bf16, or NULL with kv_len 0
+ *   kv_lens  [B] own rows of each sequence (taken as within [0, kv_len]), or
+ *            NULL: kv_len
+ *   ctx_out  [B, NH * VHD] fp32; zeros for a sequence without any key
+ * prefix_len and kv_len <= MM_MAX_KV_LEN, 0 included; B <= 2^20.  Rows past a
+ * length are not used, whatever they hold.  q, prefix and cache 16-byte aligned.
+ * Same precision as mm_mla_absorbed_decode_dev.  Device pointers, asynchronous.
+ * Workspace: `ws` of ws_bytes >= mm_mla_prefix_decode_workspace (of the same
+ * context and sizes), 16-byte aligned, device memory that no other call uses
+ * until this one is done (needed under stream capture); or NULL: the
+ * context's. */
+MM_API int mm_mla_prefix_decode_dev(mm_ctx *ctx, int layer, int B, const float *q,
+                                    const uint16_t *prefix, int prefix_len, const uint16_t *cache,
+                                    int seq_stride, const int32_t *kv_lens, int kv_len,
+                                    float *ctx_out, void *ws, size_t ws_bytes);
+MM_API int mm_mla_prefix_decode_workspace(mm_ctx *ctx, int B, int prefix_len, int kv_len,
+                                          size_t *bytes);
+
+/* The absorbed attention with a sliding window and sinks, for `rows` rows of
+ * each of B sequences: row r of sequence b is position p = kv_lens[b] - rows + r
+ * (rows = 1: the decode step's token; more: drafted tokens, a prompt's chunk)
+ * and sees the keys j <= p with j < sinks or j > p - window.  Only those rows of
+ * the cache are read.
+ *   q        [B, rows, NH, QKN + QKR] fp32, RoPE applied
+ *   cache    [B, seq_stride, KVL + QKR] bf16; its first kv_lens[b] rows, the
+ *            rows' own among them
+ *   kv_lens  [B] (taken as at most kv_len), or NULL: kv_len
+ *   ctx_out  [B, rows, NH * VHD] fp32; zeros for a row before position 0
+ * 1 <= kv_len <= MM_MAX_KV_LEN, sinks >= 0, window >= 1 (either may exceed the
+ * cache), B * rows <= 2^20.  Alignment, precision, workspace and order as
+ * mm_mla_prefix_decode_dev. */
+MM_API int mm_mla_window_decode_dev(mm_ctx *ctx, int layer, int B, int rows, const float *q,
+                                    const uint16_t *cache, int seq_stride, const int32_t *kv_lens,
+                                    int kv_len, int sinks, int window, float *ctx_out, void *ws,
+                                    size_t ws_bytes);
+MM_API int mm_mla_window_decode_workspace(mm_ctx *ctx, int B, int rows, int kv_len, int sinks,
+                                          int window, size_t *bytes);
+
 /* The absorbed chain with host pointers and the reference's own fp32 latent
  * cache (RunState kv_cache rows c_kv | k_pe, include/model.h:117):
  * q [B, NH, QKN + QKR], cache [B, seq_stride, KVL + QKR] fp32 (the first

@@ -102,6 +102,8 @@ static const struct {
     [K_F32_BF16] = {"mm_f32_bf16", MOD_UTIL},
     [K_ROUTER_WIDE] = {"mm_router_wide", MOD_MOE_BF16},
     [K_ROUTE_WIDE] = {"mm_route_wide", MOD_MOE_I8},
+    [K_MLA_ATTN_WINDOW] = {"mm_mla_attn_window", MOD_MLA},
+    [K_MLA_COMBINE_E] = {"mm_mla_combine_e", MOD_MLA},
     [K_LOGPROBS] = {"mm_logprobs", MOD_LM_HEAD},
     [K_LOGPROBS_1] = {"mm_logprobs_1", MOD_LM_HEAD},
     [K_LOGPROBS_FINAL] = {"mm_logprobs_final", MOD_LM_HEAD},

@@ -79,6 +79,8 @@ typedef enum {
     K_F32_BF16,
     K_ROUTER_WIDE,
     K_ROUTE_WIDE,
+    K_MLA_ATTN_WINDOW,
+    K_MLA_COMBINE_E,
     K_LOGPROBS,
     K_LOGPROBS_1,
     K_LOGPROBS_FINAL,

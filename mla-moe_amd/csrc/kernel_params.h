@@ -480,6 +480,10 @@ typedef struct {
     float *clat;              /* one chunk (nchunks == 1, no probabilities): clat [B, NH, KVL]
                                  written here, O / l as the merge computes it; else 0 */
     int B;
+    int pchunks;              /* chunks per (row, head group) of the partials: nchunks, or more
+                                 where other kernels write some of them */
+    int rows, sinks, window;  /* mm_mla_attn_window: rows per sequence, the keys they see */
+    int row0;                 /* mm_mla_attn_window: block row b is the call's row row0 + b */
 } mm_mla_attn_args;
 
 /* Merge the chunk partials, normalise (clat); then ctx = W_UV . clat. */

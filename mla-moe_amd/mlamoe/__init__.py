@@ -145,6 +145,12 @@ def lib():
         L.mm_mla_load_layer.argtypes = [_vp, C.c_int, _vp, C.c_uint]
         L.mm_mla_absorbed_decode_dev.argtypes = [_vp, C.c_int, C.c_int, _vp, _vp, C.c_int, _vp,
                                                  C.c_int, _vp, _vp, _vp, _vp]
+        L.mm_mla_prefix_decode_dev.argtypes = [_vp, C.c_int, C.c_int, _vp, _vp, C.c_int, _vp, C.c_int, _vp,
+                                               C.c_int, _vp, _vp, C.c_size_t]
+        L.mm_mla_prefix_decode_workspace.argtypes = [_vp, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_size_t)]
+        L.mm_mla_window_decode_dev.argtypes = [_vp, C.c_int, C.c_int, C.c_int, _vp, _vp, C.c_int, _vp, C.c_int,
+                                               C.c_int, C.c_int, _vp, _vp, C.c_size_t]
+        L.mm_mla_window_decode_workspace.argtypes = [_vp] + [C.c_int] * 5 + [C.POINTER(C.c_size_t)]
         L.mm_moe_router_logits_dev.argtypes = [_vp, C.c_int, C.c_int, _vp, _vp, _vp]
         L.mm_moe_forward_i8_debug_dev.argtypes = [_vp, C.c_int, C.c_int, _vp, _vp, _vp, _vp,
                                                   _vp, _vp, C.c_uint, C.POINTER(MoeI8Debug)]
@@ -639,6 +645,61 @@ class Context:
         _check(lib().mm_mla_absorbed_decode(self.h, layer, B, q.ctypes.data, cache.ctypes.data, L,
                                             p(lens), kv_len, ctx.ctypes.data, *[p(a) for a in outs]))
         return (ctx, *outs)
+
+    def mla_prefix_decode_dev(self, layer, B, q, prefix, prefix_len, cache, seq_stride, kv_len, ctx_out,
+                              kv_lens=None, ws=None):
+        """mm_mla_prefix_decode_dev over device buffers; ws: a DevBuf of
+        mla_prefix_decode_workspace bytes, or None for the context's."""
+        p = lambda b: None if b is None else b.ptr  # noqa: E731
+        _check(lib().mm_mla_prefix_decode_dev(self.h, layer, B, p(q), p(prefix), prefix_len, p(cache), seq_stride,
+                                              p(kv_lens), kv_len, p(ctx_out), p(ws), ws.nbytes if ws is not None else 0))
+
+    def mla_prefix_decode_workspace(self, B, prefix_len, kv_len):
+        """Bytes of workspace of a mla_prefix_decode_dev call."""
+        n = C.c_size_t()
+        _check(lib().mm_mla_prefix_decode_workspace(self.h, B, prefix_len, kv_len, C.byref(n)))
+        return n.value
+
+    def mla_prefix_decode(self, layer, q, prefix, cache, kv_lens=None):
+        """Host arrays: q [B, NH, QKN+QKR] fp32, prefix [P, KVL+QKR] and cache
+        [B, L, KVL+QKR] bf16 (uint16), either None.  Returns ctx [B, NH*VHD]."""
+        q = np.ascontiguousarray(q, np.float32)
+        up = lambda a, t: None if a is None else self.to_device(np.ascontiguousarray(a, t))  # noqa: E731
+        dq, dp, dc, dl = up(q, np.float32), up(prefix, np.uint16), up(cache, np.uint16), up(kv_lens, np.int32)
+        out = self.empty((q.shape[0], self._mla_cfg.n_heads * self._mla_cfg.v_head_dim), np.float32)
+        L = cache.shape[1] if cache is not None else 0
+        self.mla_prefix_decode_dev(layer, q.shape[0], dq, dp, prefix.shape[0] if prefix is not None else 0, dc, L, L,
+                                   out, dl)
+        got = out.download()
+        self._tmp((dq, dp, dc, dl, out))
+        return got
+
+    def mla_window_decode_dev(self, layer, B, rows, q, cache, seq_stride, kv_len, sinks, window, ctx_out,
+                              kv_lens=None, ws=None):
+        """mm_mla_window_decode_dev over device buffers; ws: a DevBuf of
+        mla_window_decode_workspace bytes, or None for the context's."""
+        p = lambda b: None if b is None else b.ptr  # noqa: E731
+        _check(lib().mm_mla_window_decode_dev(self.h, layer, B, rows, p(q), p(cache), seq_stride, p(kv_lens), kv_len,
+                                              sinks, window, p(ctx_out), p(ws), ws.nbytes if ws is not None else 0))
+
+    def mla_window_decode_workspace(self, B, rows, kv_len, sinks, window):
+        """Bytes of workspace of a mla_window_decode_dev call."""
+        n = C.c_size_t()
+        _check(lib().mm_mla_window_decode_workspace(self.h, B, rows, kv_len, sinks, window, C.byref(n)))
+        return n.value
+
+    def mla_window_decode(self, layer, q, cache, sinks, window, kv_lens=None):
+        """Host arrays: q [B, rows, NH, QKN+QKR] fp32, cache [B, L, KVL+QKR]
+        bf16 (uint16).  Returns ctx [B, rows, NH*VHD]."""
+        q = np.ascontiguousarray(q, np.float32)
+        dq, dc = self.to_device(q), self.to_device(np.ascontiguousarray(cache, np.uint16))
+        dl = None if kv_lens is None else self.to_device(np.ascontiguousarray(kv_lens, np.int32))
+        out = self.empty((*q.shape[:2], self._mla_cfg.n_heads * self._mla_cfg.v_head_dim), np.float32)
+        self.mla_window_decode_dev(layer, q.shape[0], q.shape[1], dq, dc, cache.shape[1], cache.shape[1], sinks, window,
+                                   out, dl)
+        got = out.download()
+        self._tmp((dq, dc, dl, out))
+        return got
 
     # MLA decode front -----------------------------------------------------------
     def mla_front_init(self, H, inv_freq, q_lora=0, rms_eps=1e-6, mla_eps=1e-6, interleaved=0):
