@@ -15,6 +15,7 @@ static size_t al256(size_t b) { return (b + 255) & ~(size_t)255; }
 /* A call's rows, how their keys are cut, and where its workspace holds what. */
 typedef struct {
     int R, HG;
+    int shared;                    /* the prefix by mm_mla_attn_shared */
     int pchunk, np;                /* the shared prefix: keys per chunk, chunks */
     int ochunk, no;                /* each row's own keys */
     int direct;                    /* one chunk: its blocks write clat, no merge */
@@ -35,13 +36,35 @@ static int chunk_keys(size_t blocks, int keys, int maxch) {
     return chunk;
 }
 
+/* Keys per chunk of mm_mla_attn_shared: one block per CU, so rounds of the CUs
+ * times a block's tiles (about 1.2 us of 32 keys) and its fixed part (about 7
+ * us: queries, first loads, two tiles until all roles run, its output), and 4
+ * KB per row and chunk of partials written and read back (4 TB/s). */
+static int shared_chunk_keys(int M, int keys) {
+    const int nrt = (M + 63) / 64, tiles = (keys + 31) / 32;
+    double best = 0.0;
+    int ct = tiles;
+    for (int n = 1; n <= tiles && n <= MM_MLA_MAXCH / 2; n++) {
+        const int t = (tiles + n - 1) / n, nch = (tiles + t - 1) / t;
+        const double rounds = (double)(((size_t)nrt * nch + 255) / 256);
+        const double us = rounds * (1.2 * t + 7.0) + (double)M * nch * 4096.0 / 4e6;
+        if (n == 1 || us < best) {
+            best = us;
+            ct = t;
+        }
+    }
+    return 32 * ct;
+}
+
 static void plan_decode(const mm_ctx *c, int R, int prefix, int keys, decode_plan *p) {
     const int NH = c->mla.n_heads;
     p->R = R;
     p->HG = (NH + 15) / 16;
     p->ochunk = keys > 0 ? chunk_keys((size_t)R * p->HG, keys, MM_MLA_MAXCH / 2) : 0;
     p->no = keys > 0 ? (keys + p->ochunk - 1) / p->ochunk : 0;
-    p->pchunk = prefix > 0 ? chunk_keys((size_t)R * p->HG, prefix, MM_MLA_MAXCH / 2) : 0;
+    p->shared = prefix > 0 && R * (size_t)NH >= (size_t)c->mla_shared_min;
+    p->pchunk = p->shared ? shared_chunk_keys(R * NH, prefix)
+                : prefix > 0 ? chunk_keys((size_t)R * p->HG, prefix, MM_MLA_MAXCH / 2) : 0;
     p->np = prefix > 0 ? (prefix + p->pchunk - 1) / p->pchunk : 0;
     p->direct = p->np == 0 && p->no == 1;
     const size_t row = p->direct ? 0 : (size_t)p->HG * (p->np + p->no) * (16 * MM_MLA_KVL + 32) * 4;
@@ -90,7 +113,13 @@ static int decode_run(mm_ctx *c, int layer, const decode_plan *p, const float *q
         mm_mla_attn_args a = {qhl + h0 * 2 * MM_MLA_KVL, q + h0 * (QKN + MM_MLA_QKR), NULL, NULL, 0, 0,
                               g->softmax_scale, ml, po, NULL, 0, NH, p->HG, 0, QKN, 0, NULL,
                               p->direct ? clat + h0 * MM_MLA_KVL : NULL, n, nch, 1, 0, 0, 0};
-        if (p->np) {                                  /* every row reads sequence 0 */
+        if (p->shared) {
+            const int M = n * NH;
+            mm_mla_shared_args s = {a.qhl, a.q, k->prefix, g->softmax_scale, ml, po, M, NH, p->HG, QKN,
+                                    k->prefix_len, p->pchunk, p->np, nch};
+            const unsigned nt = (unsigned)((M + 63) / 64) * (unsigned)p->np;
+            if ((st = mm_launch(c, K_MLA_ATTN_SHARED, 8 * ((nt + 7) / 8), 1, 1, 512, MM_MLA_SH_LDS, &s))) return st;
+        } else if (p->np) {                           /* every row reads sequence 0 */
             a.cache = k->prefix;
             a.kv_len = k->prefix_len;
             a.nchunks = p->np;

@@ -486,6 +486,23 @@ typedef struct {
     int row0;                 /* mm_mla_attn_window: block row b is the call's row row0 + b */
 } mm_mla_attn_args;
 
+/* Rows that all meet the same keys (mla_shared.h): blocks of 64 rows of the M =
+ * B NH and a chunk of the keys, 8 * ceil(N / 8) blocks for N = ceil(M / 64)
+ * nchunks, leaving partials as mm_mla_attn does. */
+#define MM_MLA_SHARED_MIN 1       /* rows from which it is taken */
+#define MM_MLA_SH_LDS 158720      /* dynamic LDS of a block */
+typedef struct {
+    const uint16_t *qhl;      /* [M, 2, KVL] bf16 */
+    const float *q;           /* [M, QKN + QKR] */
+    const uint16_t *keys;     /* [nkeys, KVD] bf16 */
+    float scale;
+    float *part_ml;           /* [B, HG, pchunks, 2, 16] */
+    float *part_o;            /* [B, HG, pchunks, 16, KVL] */
+    int M, NH, HG, QKN;
+    int nkeys, chunk;         /* keys per block: a multiple of 32 */
+    int nchunks, pchunks;
+} mm_mla_shared_args;
+
 /* Merge the chunk partials, normalise (clat); then ctx = W_UV . clat. */
 typedef struct {
     const float *part_ml, *part_o;
