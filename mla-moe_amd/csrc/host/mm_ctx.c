@@ -104,7 +104,8 @@ static const struct {
     [K_ROUTE_WIDE] = {"mm_route_wide", MOD_MOE_I8},
     [K_MLA_ATTN_WINDOW] = {"mm_mla_attn_window", MOD_MLA},
     [K_MLA_COMBINE_E] = {"mm_mla_combine_e", MOD_MLA},
-    [K_MLA_ATTN_SHARED] = {"mm_mla_attn_shared", MOD_MLA},
+    [K_MLA_ATTN_TILES] = {"mm_mla_attn_tiles", MOD_MLA},
+    [K_MLA_ATTN_TILES_W] = {"mm_mla_attn_tiles_w", MOD_MLA},
     [K_LOGPROBS] = {"mm_logprobs", MOD_LM_HEAD},
     [K_LOGPROBS_1] = {"mm_logprobs_1", MOD_LM_HEAD},
     [K_LOGPROBS_FINAL] = {"mm_logprobs_final", MOD_LM_HEAD},
@@ -202,11 +203,11 @@ int mm_ctx_create(int device, mm_ctx **out) {
     if (ev && *ev) c->mla_expand_min = atoi(ev);
     ev = getenv("MLAMOE_MLA_PART_MAX");
     if (ev && *ev && atoll(ev) > 0) c->mla_part_max = (size_t)atoll(ev);
-    /* MLAMOE_MLA_SHARED_MIN overrides the rows from which a shared prefix's
-     * attention takes 64-row tiles */
-    c->mla_shared_min = MM_MLA_SHARED_MIN;
-    ev = getenv("MLAMOE_MLA_SHARED_MIN");
-    if (ev && *ev) c->mla_shared_min = atoi(ev);
+    /* MLAMOE_MLA_TILES_MIN overrides the rows with common keys from which
+     * prefix and window attention takes 64-row tiles */
+    c->mla_tiles_min = MM_MLA_TILES_MIN;
+    ev = getenv("MLAMOE_MLA_TILES_MIN");
+    if (ev && *ev) c->mla_tiles_min = atoi(ev);
     /* MLAMOE_MOE_T_CHUNK lowers the rows of one MoE forward pass (longer
      * calls run in chunks of it; for testing that the chunks agree) */
     c->moe_t_chunk = 0;

@@ -81,7 +81,8 @@ typedef enum {
     K_ROUTE_WIDE,
     K_MLA_ATTN_WINDOW,
     K_MLA_COMBINE_E,
-    K_MLA_ATTN_SHARED,
+    K_MLA_ATTN_TILES,
+    K_MLA_ATTN_TILES_W,
     K_LOGPROBS,
     K_LOGPROBS_1,
     K_LOGPROBS_FINAL,
@@ -154,8 +155,9 @@ struct mm_ctx {
                                    expanded (MLAMOE_MLA_EXPAND_MIN overrides) */
     int mla_rows4;              /* row groups sharing a sequence read its keys once
                                    (MLAMOE_MLA_ROWS4=0: per row, for comparisons) */
-    int mla_shared_min;         /* rows (sequences times heads) from which a shared prefix's
-                                   attention takes 64-row tiles (MLAMOE_MLA_SHARED_MIN overrides) */
+    int mla_tiles_min;          /* rows (positions times heads) with common keys from which
+                                   prefix and window attention takes 64-row tiles
+                                   (MLAMOE_MLA_TILES_MIN overrides) */
     int moe_t_chunk;            /* cap on the rows of one MoE forward pass (0: MM_MOE_T_CHUNK) */
 
     /* growable device workspace */

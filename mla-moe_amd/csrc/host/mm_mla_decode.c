@@ -12,72 +12,6 @@ static size_t al256(size_t b) { return (b + 255) & ~(size_t)255; }
 
 #define MM_DECODE_ROWS (1 << 20)   /* rows of one call at most */
 
-/* A call's rows, how their keys are cut, and where its workspace holds what. */
-typedef struct {
-    int R, HG;
-    int shared;                    /* the prefix by mm_mla_attn_shared */
-    int pchunk, np;                /* the shared prefix: keys per chunk, chunks */
-    int ochunk, no;                /* each row's own keys */
-    int direct;                    /* one chunk: its blocks write clat, no merge */
-    int G;                         /* rows whose partials are held at once */
-    size_t o_qhl, o_clat, o_ml, o_po, bytes;
-} decode_plan;
-
-/* Keys per chunk: as decode_rows (mm_mla.c), MM_MLA_CHUNK halved while the
- * grid has fewer than MM_MLA_MIN_BLOCKS blocks and a row at most 64 chunks;
- * doubled where a row would have more than maxch. */
-static int chunk_keys(size_t blocks, int keys, int maxch) {
-    int chunk = MM_MLA_CHUNK;
-    while (chunk > 16 * MM_MLA_AW && blocks * ((keys + chunk - 1) / chunk) < MM_MLA_MIN_BLOCKS &&
-           (keys + chunk / 2 - 1) / (chunk / 2) <= 64)
-        chunk /= 2;
-    if (chunk < MM_MLA_CHUNK && keys > chunk && keys <= chunk + chunk / 2) chunk *= 2;
-    while ((keys + chunk - 1) / chunk > maxch) chunk *= 2;
-    return chunk;
-}
-
-/* Keys per chunk of mm_mla_attn_shared: one block per CU, so rounds of the CUs
- * times a block's tiles (about 1.2 us of 32 keys) and its fixed part (about 7
- * us: queries, first loads, two tiles until all roles run, its output), and 4
- * KB per row and chunk of partials written and read back (4 TB/s). */
-static int shared_chunk_keys(int M, int keys) {
-    const int nrt = (M + 63) / 64, tiles = (keys + 31) / 32;
-    double best = 0.0;
-    int ct = tiles;
-    for (int n = 1; n <= tiles && n <= MM_MLA_MAXCH / 2; n++) {
-        const int t = (tiles + n - 1) / n, nch = (tiles + t - 1) / t;
-        const double rounds = (double)(((size_t)nrt * nch + 255) / 256);
-        const double us = rounds * (1.2 * t + 7.0) + (double)M * nch * 4096.0 / 4e6;
-        if (n == 1 || us < best) {
-            best = us;
-            ct = t;
-        }
-    }
-    return 32 * ct;
-}
-
-static void plan_decode(const mm_ctx *c, int R, int prefix, int keys, decode_plan *p) {
-    const int NH = c->mla.n_heads;
-    p->R = R;
-    p->HG = (NH + 15) / 16;
-    p->ochunk = keys > 0 ? chunk_keys((size_t)R * p->HG, keys, MM_MLA_MAXCH / 2) : 0;
-    p->no = keys > 0 ? (keys + p->ochunk - 1) / p->ochunk : 0;
-    p->shared = prefix > 0 && R * (size_t)NH >= (size_t)c->mla_shared_min;
-    p->pchunk = p->shared ? shared_chunk_keys(R * NH, prefix)
-                : prefix > 0 ? chunk_keys((size_t)R * p->HG, prefix, MM_MLA_MAXCH / 2) : 0;
-    p->np = prefix > 0 ? (prefix + p->pchunk - 1) / p->pchunk : 0;
-    p->direct = p->np == 0 && p->no == 1;
-    const size_t row = p->direct ? 0 : (size_t)p->HG * (p->np + p->no) * (16 * MM_MLA_KVL + 32) * 4;
-    p->G = R;
-    if (row && (size_t)R * row > c->mla_part_max) p->G = c->mla_part_max / row > 0 ? (int)(c->mla_part_max / row) : 1;
-    p->o_qhl = 0;
-    p->o_clat = al256((size_t)R * NH * 2 * MM_MLA_KVL * 2);
-    p->o_ml = p->o_clat + al256((size_t)R * NH * MM_MLA_KVL * 4);
-    const size_t parts = p->direct ? 0 : (size_t)p->G * p->HG * (p->np + p->no);
-    p->o_po = p->o_ml + al256(parts * 32 * 4);
-    p->bytes = p->o_po + al256(parts * 16 * MM_MLA_KVL * 4);
-}
-
 /* The rows' keys: a prefix all of them read, and / or windows of their sequences'
  * caches, `rows` rows per sequence (one row and a window of kv_len: the cache). */
 typedef struct {
@@ -88,7 +22,154 @@ typedef struct {
     const int32_t *kv_lens;
     int kv_len;                    /* the longest cache */
     int rows, sinks, window;
+    int own;                       /* keys of its own that a row (64 rows together) sees at most */
 } decode_keys;
+
+/* A call's rows, how their keys are cut, and where its workspace holds what. */
+typedef struct {
+    int R, HG;
+    int tiles;                     /* 64 rows per block (mla_tiles.h), else 16 */
+    int pchunk, np;                /* the prefix: keys per chunk, chunks */
+    int ochunk, no;                /* own keys */
+    int direct;                    /* one chunk of 16-row blocks: they write clat, no merge */
+    int G;                         /* rows whose partials are held at once */
+    size_t o_qhl, o_clat, o_ml, o_po, bytes;
+} decode_plan;
+
+/* Keys per chunk of the 16-row blocks: as decode_rows (mm_mla.c), MM_MLA_CHUNK
+ * halved while the grid has fewer than MM_MLA_MIN_BLOCKS blocks and a row at most
+ * 64 chunks; doubled where a row would have more than maxch. */
+static int chunk_keys(size_t blocks, int keys, int maxch) {
+    int chunk = MM_MLA_CHUNK;
+    while (chunk > 16 * MM_MLA_AW && blocks * ((keys + chunk - 1) / chunk) < MM_MLA_MIN_BLOCKS &&
+           (keys + chunk / 2 - 1) / (chunk / 2) <= 64)
+        chunk /= 2;
+    if (chunk < MM_MLA_CHUNK && keys > chunk && keys <= chunk + chunk / 2) chunk *= 2;
+    while ((keys + chunk - 1) / chunk > maxch) chunk *= 2;
+    return chunk;
+}
+
+/* Chunks of the 64-row blocks, one block per CU: us of a block with t tiles of 32
+ * keys over 64 (or up to 32) rows -- queries, first loads, two tiles until all
+ * roles run, its output --, and of the partials written and read back (4 KB per
+ * row and chunk at 4 TB/s). */
+static double tiles_us(int t, int nrows) { return (nrows > 32 ? 1.9 : 1.2) * t + 9.0; }
+
+static void tiles_chunks(int R, int NH, int rows, int prefix, int own, decode_plan *p) {
+    const size_t nrt = ((size_t)R * NH + 63) / 64, ort = (size_t)(R / rows) * ((rows * NH + 63) / 64);
+    const int pt = (prefix + 31) / 32, ot = (own + 31) / 32, most = MM_MLA_MAXCH / 2;
+    double best = -1.0;
+    for (int n = 1; n <= (pt > 0 ? pt : ot) && n <= most; n++) {
+        int t, u, np = 0, no = 0;
+        if (pt > 0) {               /* own chunks as long as the prefix's, so that they fill in beside */
+            t = (pt + n - 1) / n;
+            u = t < ot ? t : ot;
+        } else {
+            t = 0;
+            u = (ot + n - 1) / n;
+        }
+        if (u > 0 && (ot + u - 1) / u > most) u = (ot + most - 1) / most;
+        if (t > 0) np = (pt + t - 1) / t;
+        if (u > 0) no = (ot + u - 1) / u;
+        const double lp = np ? tiles_us(t, 64) : 0.0, lo = no ? tiles_us(u, rows * NH) : 0.0;
+        /* the prefix's blocks in rounds of the CUs, the own ones into what the
+         * last round leaves, then in rounds */
+        const size_t bp = nrt * np, bo = ort * no, q = bp / 256, r = bp % 256;
+        size_t room = 0;
+        if (r && bo) room = (256 - r) * (lp >= lo ? (size_t)(lp / lo) : 0);
+        const size_t rest = bo > room ? bo - room : 0;
+        double us = (double)(q + (r > 0)) * lp + (double)((rest + 255) / 256) * lo;
+        us += (double)R * NH * (np + no) * 4096.0 / 4e6;
+        if (best < 0.0 || us < best) {
+            best = us;
+            p->pchunk = 32 * t;
+            p->np = np;
+            p->ochunk = 32 * u;
+            p->no = no;
+        }
+    }
+}
+
+static void plan_decode(const mm_ctx *c, int R, const decode_keys *k, decode_plan *p) {
+    const int NH = c->mla.n_heads;
+    p->R = R;
+    p->HG = (NH + 15) / 16;
+    p->pchunk = p->np = p->ochunk = p->no = 0;
+    /* rows that meet the same keys */
+    p->tiles = (k->prefix_len > 0 ? (size_t)R * NH : (size_t)k->rows * NH) >= (size_t)c->mla_tiles_min;
+    int unit = 1;                  /* rows that fill whole tiles */
+    if (p->tiles) {
+        tiles_chunks(R, NH, k->rows, k->prefix_len, k->own, p);
+        while ((unit * NH) % 64) unit++;
+    } else {
+        const int own = k->own < k->sinks + k->window ? k->own : k->sinks + k->window;
+        if (own > 0) p->ochunk = chunk_keys((size_t)R * p->HG, own, MM_MLA_MAXCH / 2);
+        if (own > 0) p->no = (own + p->ochunk - 1) / p->ochunk;
+        if (k->prefix_len > 0) p->pchunk = chunk_keys((size_t)R * p->HG, k->prefix_len, MM_MLA_MAXCH / 2);
+        if (k->prefix_len > 0) p->np = (k->prefix_len + p->pchunk - 1) / p->pchunk;
+    }
+    p->direct = !p->tiles && p->np == 0 && p->no == 1;
+    const size_t row = p->direct ? 0 : (size_t)p->HG * (p->np + p->no) * (16 * MM_MLA_KVL + 32) * 4;
+    p->G = R;
+    if (row && (size_t)R * row > c->mla_part_max) {
+        const size_t g = c->mla_part_max / row / unit * unit;
+        p->G = g > 0 ? (int)g : unit;
+    }
+    p->o_qhl = 0;
+    p->o_clat = al256((size_t)R * NH * 2 * MM_MLA_KVL * 2);
+    p->o_ml = p->o_clat + al256((size_t)R * NH * MM_MLA_KVL * 4);
+    const size_t parts = p->direct ? 0 : (size_t)(p->G < R ? p->G : R) * p->HG * (p->np + p->no);
+    p->o_po = p->o_ml + al256(parts * 32 * 4);
+    p->bytes = p->o_po + al256(parts * 16 * MM_MLA_KVL * 4);
+}
+
+/* Rows r0 .. r0 + n - 1 of the call: their attention partials (or clat). */
+static int attend_16(mm_ctx *c, const decode_plan *p, const decode_keys *k, const uint16_t *qhl, const float *q,
+                     int r0, int n, float *clat, float *ml, float *po) {
+    const mm_mla_config *g = &c->mla;
+    const int NH = g->n_heads, nch = p->np + p->no;
+    const size_t alds = (size_t)MM_MLA_AW * 2 * MM_MLA_TILE_B;
+    int st;
+    mm_mla_attn_args a = {qhl, q, NULL, NULL, 0, 0, g->softmax_scale, ml, po, NULL, 0, NH, p->HG, 0,
+                          g->qk_nope_head_dim, 0, NULL, p->direct ? clat : NULL, n, nch, 1, 0, 0, 0};
+    if (p->np) {                                      /* every row reads sequence 0 */
+        a.cache = k->prefix;
+        a.kv_len = k->prefix_len;
+        a.nchunks = p->np;
+        a.chunk = p->pchunk;
+        const unsigned nt = (unsigned)n * (unsigned)p->HG * (unsigned)p->np;
+        if ((st = mm_launch(c, K_MLA_ATTN, 8 * ((nt + 7) / 8), 1, 1, 64 * MM_MLA_AW, alds, &a))) return st;
+    }
+    if (!p->no) return MM_OK;
+    a.cache = k->cache;
+    a.seq_stride = k->seq_stride;
+    a.kv_lens = k->kv_lens;
+    a.kv_len = k->kv_len;
+    a.nchunks = p->no;
+    a.chunk = p->ochunk;
+    a.rows = k->rows;
+    a.sinks = k->sinks;
+    a.window = k->window;
+    a.row0 = r0;
+    a.part_ml = ml + (size_t)p->np * 32;
+    a.part_o = po + (size_t)p->np * 16 * MM_MLA_KVL;
+    const unsigned nt = (unsigned)n * (unsigned)p->HG * (unsigned)p->no;
+    return mm_launch(c, K_MLA_ATTN_WINDOW, 8 * ((nt + 7) / 8), 1, 1, 64 * MM_MLA_AW, alds, &a);
+}
+
+/* The same in 64-row blocks; the rows are whole sequences, or part of one. */
+static int attend_64(mm_ctx *c, const decode_plan *p, const decode_keys *k, const uint16_t *qhl, const float *q,
+                     int r0, int n, float *ml, float *po) {
+    const mm_mla_config *g = &c->mla;
+    const int NH = g->n_heads, M = n * NH, rows = n < k->rows ? n : k->rows, nseq = n / rows;
+    mm_mla_tiles_args a = {qhl, q, g->softmax_scale, ml, po, M, NH, p->HG, g->qk_nope_head_dim, p->np + p->no,
+                           k->prefix, k->prefix_len, p->pchunk, p->np, k->cache, k->kv_lens, k->kv_len, k->seq_stride,
+                           r0 / k->rows, nseq, rows, p->ochunk, p->no, k->rows, r0 % k->rows, k->sinks, k->window};
+    const unsigned np = (unsigned)((M + 63) / 64) * (unsigned)p->np;
+    const unsigned no = (unsigned)nseq * (unsigned)((rows * NH + 63) / 64) * (unsigned)p->no;
+    return mm_launch(c, p->np || (k->rows == 1 && k->window >= k->kv_len) ? K_MLA_ATTN_TILES : K_MLA_ATTN_TILES_W,
+                     8 * ((np + 7) / 8) + 8 * ((no + 7) / 8), 1, 1, 512, MM_MLA_TL_LDS, &a);
+}
 
 static int decode_run(mm_ctx *c, int layer, const decode_plan *p, const float *q, const decode_keys *k,
                       float *ctx_out, char *ws) {
@@ -103,53 +184,27 @@ static int decode_run(mm_ctx *c, int layer, const decode_plan *p, const float *q
     int st = mm_launch(c, wide ? K_MLA_QPREP_W : K_MLA_QPREP, MM_MLA_KVL / (wide ? 64 * MM_MLA_WIDE_S : 64),
                        (unsigned)NH, rt, 256, 0, &qa);
     if (st) return st;
-    const int nch = p->np + p->no;
-    const size_t alds = (size_t)MM_MLA_AW * 2 * MM_MLA_TILE_B;
     mm_mla_combine_args ca = {ml, po, kv_b, NULL, 0, ctx_out, clat, NULL, 0, R, NH, QKN, g->v_head_dim,
-                              p->HG, nch, NULL};
-    for (int r0 = 0; r0 < R; r0 += p->G) {
-        const int n = R - r0 < p->G ? R - r0 : p->G;
+                              p->HG, p->np + p->no, NULL};
+    for (int r0 = 0, n; r0 < R; r0 += n) {
+        n = R - r0 < p->G ? R - r0 : p->G;
+        if (p->tiles && k->rows > 1 && n < R) {       /* whole sequences, or within one */
+            const int left = k->rows - r0 % k->rows;
+            if (r0 % k->rows == 0 && n >= k->rows) n = n / k->rows * k->rows;
+            else if (n > left) n = left;
+        }
         const size_t h0 = (size_t)r0 * NH;
-        mm_mla_attn_args a = {qhl + h0 * 2 * MM_MLA_KVL, q + h0 * (QKN + MM_MLA_QKR), NULL, NULL, 0, 0,
-                              g->softmax_scale, ml, po, NULL, 0, NH, p->HG, 0, QKN, 0, NULL,
-                              p->direct ? clat + h0 * MM_MLA_KVL : NULL, n, nch, 1, 0, 0, 0};
-        if (p->shared) {
-            const int M = n * NH;
-            mm_mla_shared_args s = {a.qhl, a.q, k->prefix, g->softmax_scale, ml, po, M, NH, p->HG, QKN,
-                                    k->prefix_len, p->pchunk, p->np, nch};
-            const unsigned nt = (unsigned)((M + 63) / 64) * (unsigned)p->np;
-            if ((st = mm_launch(c, K_MLA_ATTN_SHARED, 8 * ((nt + 7) / 8), 1, 1, 512, MM_MLA_SH_LDS, &s))) return st;
-        } else if (p->np) {                           /* every row reads sequence 0 */
-            a.cache = k->prefix;
-            a.kv_len = k->prefix_len;
-            a.nchunks = p->np;
-            a.chunk = p->pchunk;
-            const unsigned nt = (unsigned)n * (unsigned)p->HG * (unsigned)p->np;
-            if ((st = mm_launch(c, K_MLA_ATTN, 8 * ((nt + 7) / 8), 1, 1, 64 * MM_MLA_AW, alds, &a))) return st;
-        }
-        if (p->no) {
-            a.cache = k->cache;
-            a.seq_stride = k->seq_stride;
-            a.kv_lens = k->kv_lens;
-            a.kv_len = k->kv_len;
-            a.nchunks = p->no;
-            a.chunk = p->ochunk;
-            a.rows = k->rows;
-            a.sinks = k->sinks;
-            a.window = k->window;
-            a.row0 = r0;
-            a.part_ml = ml + (size_t)p->np * 32;
-            a.part_o = po + (size_t)p->np * 16 * MM_MLA_KVL;
-            const unsigned nt = (unsigned)n * (unsigned)p->HG * (unsigned)p->no;
-            if ((st = mm_launch(c, K_MLA_ATTN_WINDOW, 8 * ((nt + 7) / 8), 1, 1, 64 * MM_MLA_AW, alds, &a))) return st;
-        }
-        if (!p->direct) {
-            mm_mla_combine_args cg = ca;
-            cg.clat = clat + h0 * MM_MLA_KVL;
-            cg.B = n;
-            const unsigned z = (size_t)NH * R < 128 ? MM_MLA_KVL / 128 : 1;
-            if ((st = mm_launch(c, K_MLA_COMBINE_E, (unsigned)NH, (unsigned)n, z, 256, 0, &cg))) return st;
-        }
+        const uint16_t *qh = qhl + h0 * 2 * MM_MLA_KVL;
+        const float *qr = q + h0 * (QKN + MM_MLA_QKR);
+        float *cl = clat + h0 * MM_MLA_KVL;
+        st = p->tiles ? attend_64(c, p, k, qh, qr, r0, n, ml, po) : attend_16(c, p, k, qh, qr, r0, n, cl, ml, po);
+        if (st) return st;
+        if (p->direct) continue;
+        mm_mla_combine_args cg = ca;
+        cg.clat = cl;
+        cg.B = n;
+        const unsigned z = (size_t)NH * R < 128 ? MM_MLA_KVL / 128 : 1;
+        if ((st = mm_launch(c, K_MLA_COMBINE_E, (unsigned)NH, (unsigned)n, z, 256, 0, &cg))) return st;
     }
     const int vt = wide ? 16 * MM_MLA_WIDE_S : 16;
     return mm_launch(c, wide ? K_MLA_UV_W : K_MLA_UV, (unsigned)((g->v_head_dim + vt - 1) / vt), (unsigned)NH, rt,
@@ -167,13 +222,20 @@ static int prefix_check(const mm_ctx *c, const char *name, int B, int prefix_len
     return MM_OK;
 }
 
+static decode_keys prefix_keys(const uint16_t *prefix, int prefix_len, const uint16_t *cache, int seq_stride,
+                               const int32_t *kv_lens, int kv_len) {
+    const decode_keys k = {prefix, prefix_len, cache, seq_stride, kv_lens, kv_len, 1, 0, kv_len, kv_len};
+    return k;
+}
+
 int mm_mla_prefix_decode_workspace(mm_ctx *c, int B, int prefix_len, int kv_len, size_t *bytes) {
     if (!bytes) return mm_fail(MM_ERR_INVALID, "mm_mla_prefix_decode_workspace: NULL argument");
     *bytes = 0;
     const int st = prefix_check(c, "mm_mla_prefix_decode_workspace", B, prefix_len, kv_len);
     if (st || B == 0) return st;
+    const decode_keys k = prefix_keys(NULL, prefix_len, NULL, kv_len, NULL, kv_len);
     decode_plan p;
-    plan_decode(c, B, prefix_len, kv_len, &p);
+    plan_decode(c, B, &k, &p);
     *bytes = p.bytes;
     return MM_OK;
 }
@@ -194,11 +256,11 @@ int mm_mla_prefix_decode_dev(mm_ctx *c, int layer, int B, const float *q, const 
     if ((prefix_len && (uintptr_t)prefix % 16) || (kv_len && (uintptr_t)cache % 16) || (uintptr_t)q % 16)
         return mm_fail(MM_ERR_INVALID, "%s: q, prefix and cache must be 16-byte aligned", name);
     if ((st = mm_set_device(c))) return st;
+    const decode_keys k = prefix_keys(prefix, prefix_len, cache, seq_stride, kv_lens, kv_len);
     decode_plan p;
-    plan_decode(c, B, prefix_len, kv_len, &p);
+    plan_decode(c, B, &k, &p);
     char *w;
     if ((st = mm_call_workspace(c, name, ws, ws_bytes, p.bytes, (void **)&w))) return st;
-    const decode_keys k = {prefix, prefix_len, cache, seq_stride, kv_lens, kv_len, 1, 0, kv_len};
     return decode_run(c, layer, &p, q, &k, ctx_out, w);
 }
 
@@ -214,11 +276,17 @@ static int window_check(const mm_ctx *c, const char *name, int B, int rows, int 
     return MM_OK;
 }
 
-/* Keys that a row sees at most (both no longer than the cache: no overflow). */
-static int window_keys(int kv_len, int *sinks, int *window) {
-    if (*sinks > kv_len) *sinks = kv_len;
-    if (*window > kv_len) *window = kv_len;
-    return *sinks + *window < kv_len ? *sinks + *window : kv_len;
+/* sinks and window no longer than the cache; the keys that the rows of a tile
+ * (as many positions as 64 rows touch) see at most. */
+static decode_keys window_keys(const mm_ctx *c, int rows, const uint16_t *cache, int seq_stride,
+                               const int32_t *kv_lens, int kv_len, int sinks, int window) {
+    if (sinks > kv_len) sinks = kv_len;
+    if (window > kv_len) window = kv_len;
+    int span = 64 / c->mla.n_heads + 2;
+    if (span > rows) span = rows;
+    const int own = sinks + window + span - 1;
+    const decode_keys k = {NULL, 0, cache, seq_stride, kv_lens, kv_len, rows, sinks, window, own < kv_len ? own : kv_len};
+    return k;
 }
 
 int mm_mla_window_decode_workspace(mm_ctx *c, int B, int rows, int kv_len, int sinks, int window, size_t *bytes) {
@@ -226,8 +294,9 @@ int mm_mla_window_decode_workspace(mm_ctx *c, int B, int rows, int kv_len, int s
     *bytes = 0;
     const int st = window_check(c, "mm_mla_window_decode_workspace", B, rows, kv_len, sinks, window);
     if (st || B == 0) return st;
+    const decode_keys k = window_keys(c, rows, NULL, kv_len, NULL, kv_len, sinks, window);
     decode_plan p;
-    plan_decode(c, B * rows, 0, window_keys(kv_len, &sinks, &window), &p);
+    plan_decode(c, B * rows, &k, &p);
     *bytes = p.bytes;
     return MM_OK;
 }
@@ -246,11 +315,10 @@ int mm_mla_window_decode_dev(mm_ctx *c, int layer, int B, int rows, const float 
     if ((uintptr_t)cache % 16 || (uintptr_t)q % 16)
         return mm_fail(MM_ERR_INVALID, "%s: q and cache must be 16-byte aligned", name);
     if ((st = mm_set_device(c))) return st;
-    const int keys = window_keys(kv_len, &sinks, &window);
+    const decode_keys k = window_keys(c, rows, cache, seq_stride, kv_lens, kv_len, sinks, window);
     decode_plan p;
-    plan_decode(c, B * rows, 0, keys, &p);
+    plan_decode(c, B * rows, &k, &p);
     char *w;
     if ((st = mm_call_workspace(c, name, ws, ws_bytes, p.bytes, (void **)&w))) return st;
-    const decode_keys k = {NULL, 0, cache, seq_stride, kv_lens, kv_len, rows, sinks, window};
     return decode_run(c, layer, &p, q, &k, ctx_out, w);
 }

@@ -486,22 +486,31 @@ typedef struct {
     int row0;                 /* mm_mla_attn_window: block row b is the call's row row0 + b */
 } mm_mla_attn_args;
 
-/* Rows that all meet the same keys (mla_shared.h): blocks of 64 rows of the M =
- * B NH and a chunk of the keys, 8 * ceil(N / 8) blocks for N = ceil(M / 64)
- * nchunks, leaving partials as mm_mla_attn does. */
-#define MM_MLA_SHARED_MIN 1       /* rows from which it is taken */
-#define MM_MLA_SH_LDS 158720      /* dynamic LDS of a block */
+/* Rows that meet common keys (mla_tiles.h): blocks of 64 rows (position, head)
+ * and a chunk of the keys, leaving partials as mm_mla_attn does.  A 1-D grid:
+ * 8 * ceil(N / 8) blocks for the N = ceil(M / 64) nchunks of the prefix (none
+ * where nchunks is 0), then as many for the N = nseq ceil(rows NH / 64)
+ * ochunks of the sequences' own keys. */
+#define MM_MLA_TL_LDS 158720      /* dynamic LDS of a block */
+#define MM_MLA_TILES_MIN 1        /* rows from which they are taken */
 typedef struct {
     const uint16_t *qhl;      /* [M, 2, KVL] bf16 */
     const float *q;           /* [M, QKN + QKR] */
-    const uint16_t *keys;     /* [nkeys, KVD] bf16 */
     float scale;
-    float *part_ml;           /* [B, HG, pchunks, 2, 16] */
-    float *part_o;            /* [B, HG, pchunks, 16, KVL] */
-    int M, NH, HG, QKN;
-    int nkeys, chunk;         /* keys per block: a multiple of 32 */
-    int nchunks, pchunks;
-} mm_mla_shared_args;
+    float *part_ml;           /* [M / NH, HG, pchunks, 2, 16] */
+    float *part_o;            /* [M / NH, HG, pchunks, 16, KVL] */
+    int M, NH, HG, QKN, pchunks;
+    const uint16_t *keys;     /* [nkeys, KVD] bf16: the prefix */
+    int nkeys, chunk, nchunks;   /* keys per block: a multiple of 32 */
+    const uint16_t *cache;    /* [sequences, seq_stride, KVD] bf16 */
+    const int32_t *kv_lens;   /* [sequences] or 0 */
+    int kv_len, seq_stride;
+    int seq0, nseq, rows;     /* sequences seq0 .. seq0 + nseq - 1, `rows` rows of each */
+    int ochunk, ochunks;      /* partials nchunks .. nchunks + ochunks - 1 */
+    /* mm_mla_attn_tiles_w: row r of sequence s is position kv_lens[s] - all_rows
+     * + roff + r */
+    int all_rows, roff, sinks, window;
+} mm_mla_tiles_args;
 
 /* Merge the chunk partials, normalise (clat); then ctx = W_UV . clat. */
 typedef struct {

@@ -16,6 +16,8 @@
  *   mm_mla_combine  merge the chunk partials, clat = O / l
  *   mm_mla_uv       ctx = W_UV . clat
  */
+#include <type_traits>
+
 #include "common.h"
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -880,7 +882,7 @@ extern "C" __global__ __launch_bounds__(AW * MM_WAVE) void mm_mla_attn_rows(mm_m
 }
 
 #include "mla_expand.h"
-#include "mla_shared.h"
+#include "mla_tiles.h"
 
 /* Merge the chunk partials of (head h, sequence b): clat = sum_c w_c O_c / l
  * with w_c = e^(m_c - m); also turns the debug scores into probabilities.

@@ -1,0 +1,463 @@
+/* mla_tiles.h -- absorbed MLA attention of many rows over common keys (part of
+ * mla.hip): the prefix that a decode batch shares with each sequence's own keys,
+ * and the rows of a prompt's chunk through a sliding window.
+ *
+ * A row is one (position, head).  It costs 1,088 products a key, twice over since
+ * the fp32 query and the probabilities travel as bf16 pairs.  mm_mla_attn keeps 16
+ * rows (one position's heads) per wave, so that each position reads its keys for
+ * itself and 16 x 16 tiles are fed from LDS once per 16 rows.  Here a block takes
+ * 64 rows over a chunk of their keys on 32 x 32 tiles, one block per CU, its eight
+ * waves in three roles (each SIMD holds one of the first four and one of the
+ * last), each one 32-key tile behind the other:
+ *   waves 0, 1   scores of tile t + 2 over latents 0..287 (32 rows each)
+ *   waves 2, 3   scores of tile t + 1 over latents 288..575, added to the former;
+ *                softmax; the probabilities as bf16 pairs to LDS
+ *   waves 4..7   O += P V of tile t, 64 rows x 128 latent columns each; and the
+ *                loads of the tiles to come
+ * A score wave keeps its 32 rows' queries over its half of the latents (144
+ * registers), an output wave its 64 x 128 of O (128 registers): neither would
+ * fit beside the other, and the softmax of one tile runs beside the products of
+ * the others.  One barrier per tile.
+ *
+ * LDS, per tile of 32 keys: latents 0..287 (576 bytes a row, four tiles of
+ * them), 288..511 (448 bytes, three), k_pe (128 bytes, two): a part lives until
+ * its last reader.  Rows are 16-byte pieces, piece p of row r in slot p with its
+ * low two bits exclusive-ored with r / 4: a wave's reads (32 rows of one piece, or
+ * four rows of a 32-column stretch, transposing) then fall on all banks, since
+ * both row lengths are odd multiples of 64 bytes.  Rows past the keys are
+ * beyond the buffer's range: zeros, no read; their scores are masked.
+ *
+ * Key order inside a 16-key step of P and V: half h of the lanes holds keys 4 h
+ * + {0..3, 8..11}, the keys of its registers after the score product. */
+#define TL_R0 18432                /* bytes of one tile: latents 0..287 */
+#define TL_R1 14336                /* latents 288..511 */
+#define TL_KP 4096                 /* k_pe */
+#define TL_O1 (4 * TL_R0)
+#define TL_OK (TL_O1 + 3 * TL_R1)
+#define TL_OP (TL_OK + 2 * TL_KP)  /* P: two tiles of 64 rows x 32 keys, hi then lo */
+#define TL_OX (TL_OP + 2 * 8192)   /* partial scores: two tiles of 64 x 32 floats */
+#define TL_OF (TL_OX + 2 * 8192)   /* rescaling factors: two tiles of 64 floats */
+#define TL_OG (TL_OF + 2 * 256)    /* [tile % 2][row half]: whether there are some; keys that are not finite */
+#define TL_OT (TL_OG + 32)         /* 64 rows' places in the partials */
+static_assert(TL_OT + 256 <= MM_MLA_TL_LDS && MM_MLA_TL_LDS <= 163840, "LDS of a block");
+typedef __attribute__((address_space(3))) s16x4 *lds_s4;
+typedef __attribute__((address_space(3))) i32x4 *lds_w4;
+typedef __attribute__((address_space(3))) f32x4 *lds_f4;
+typedef __attribute__((address_space(3))) float *lds_f;
+typedef __attribute__((address_space(3))) int *lds_i;
+
+/* LDS accesses done, then the block's barrier; loads into LDS stay in flight. */
+__device__ __forceinline__ void tl_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+/* A block's rows and keys. */
+struct tl_job {
+    const uint16_t *keys;          /* first of the chunk's keys; WIN: the sequence's cache */
+    int row0, nrows;               /* flat rows (position, head) of the call */
+    int chunk;                     /* its place among a row's partials */
+    int nk;                        /* keys of the chunk */
+    /* WIN: the chunk's key v is key v0 + v of the tile's list: the sinks, then
+     * from `sinks` on shifted to where the first row's window begins */
+    int v0, len, shift, first_row, pos0;   /* pos0: position of the sequence's row 0 in this launch */
+};
+
+/* WIN: key of list entry v */
+__device__ __forceinline__ int tl_key(const mm_mla_tiles_args &a, const tl_job &j, int v) {
+    return v + (v >= a.sinks ? j.shift : 0);
+}
+
+template <bool WIN>
+__device__ __forceinline__ bool tl_find(const mm_mla_tiles_args &a, tl_job &j) {
+    /* both lists in eighths, one per XCD, neighbours (which read the same keys)
+     * from one L2: the prefix's blocks chunk by chunk, then the sequences' own */
+    const int nrt = (a.M + 63) / 64, nsh = nrt * a.nchunks, psh = (nsh + 7) / 8;
+    int i = (int)blockIdx.x;
+    if (!WIN && i < 8 * psh) {
+        const int trip = i % 8 * psh + i / 8;
+        if (trip >= nsh) return false;
+        j.chunk = trip / nrt;
+        j.row0 = trip % nrt * 64;
+        j.nrows = min(64, a.M - j.row0);
+        const int k0 = j.chunk * a.chunk;
+        j.nk = min(a.chunk, a.nkeys - k0);
+        j.keys = a.keys + (size_t)k0 * KVD;
+        return true;
+    }
+    i -= WIN ? 0 : 8 * psh;
+    const int rn = a.rows * a.NH, nt = (rn + 63) / 64, nown = a.nseq * nt * a.ochunks, po = (nown + 7) / 8;
+    const int trip = i % 8 * po + i / 8;
+    if (i >= 8 * po || trip >= nown) return false;
+    const int c = trip % a.ochunks, tile = trip / a.ochunks % nt, s = trip / (a.ochunks * nt);
+    const int seq = a.seq0 + s;
+    const int L = max(min(a.kv_lens ? a.kv_lens[seq] : a.kv_len, a.kv_len), 0);
+    j.first_row = 64 * tile;
+    j.nrows = min(64, rn - j.first_row);
+    j.row0 = s * rn + j.first_row;
+    j.chunk = a.nchunks + c;
+    j.keys = a.cache + (size_t)seq * a.seq_stride * KVD;
+    j.v0 = c * a.ochunk;
+    int n = L;
+    if (WIN) {
+        j.len = L;
+        j.pos0 = L - a.all_rows + a.roff;
+        const int pa = j.pos0 + j.first_row / a.NH, pb = j.pos0 + (j.first_row + j.nrows - 1) / a.NH;
+        const int lo = max(pa - a.window + 1, 0);      /* the first row's window */
+        j.shift = lo > a.sinks ? lo - a.sinks : 0;
+        n = max(pb + 1 - j.shift, 0);
+    } else {
+        j.keys += (size_t)min(j.v0, L) * KVD;
+    }
+    j.nk = min(max(n - j.v0, 0), a.ochunk);
+    return true;
+}
+
+template <bool WIN>
+__device__ __forceinline__ void tl_block(const mm_mla_tiles_args &a) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t slds[];
+    const uint32_t lds0 = lds_addr(slds);
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c32 = lane & 31, hi = lane >> 5;
+    tl_job j;
+    if (!tl_find<WIN>(a, j)) return;
+    const int nt = (j.nk + 31) / 32;
+    const bool two = j.nrows > 32;                     /* rows in both halves */
+    if (tid < 64) {                                    /* row (b, h): partial ((b HG + h / 16) pchunks + chunk), line h % 16 */
+        const int r = j.row0 + min(tid, j.nrows - 1), b = r / a.NH, h = r - b * a.NH;
+        ((lds_i)(uintptr_t)(lds0 + TL_OT))[tid] = ((b * a.HG + (h >> 4)) * a.pchunks + j.chunk) * 16 + (h & 15);
+    }
+
+    if (w >= 4) {
+        /* ---- O += P V, and the loads ---- */
+        const int bw = w - 4;
+        const rsrc_t rk = raw_rsrc(j.keys, (uint32_t)(WIN ? j.len : j.nk) * KVD * 2);
+        /* this wave's nine of a tile's 36 1-KB loads: LDS piece x (16 bytes) of
+         * the part is row x / pieces-per-row, slot x % it */
+        uint32_t so[9], dl[9];
+        int kr[9];                                     /* WIN: the row */
+#pragma unroll
+        for (int i = 0; i < 9; i++) {
+            const bool r0 = i < 4 || (i == 4 && bw < 2);
+            const int u = i < 4 ? bw + 4 * i : i == 4 ? (bw < 2 ? 16 + bw : 10 + bw) : i < 8 ? bw + 4 * (i - 5) : bw;
+            const int x = 64 * u + lane;
+            int r, o;
+            if (i == 8) {
+                r = x >> 3;
+                o = KVL * 2 + 16 * ((x & 7) ^ ((r >> 1) & 7));
+            } else {
+                const int ppr = r0 ? 36 : 28;
+                r = x / ppr;
+                const int s = x - r * ppr;
+                o = (r0 ? 0 : 576) + 16 * ((s & ~3) | ((s ^ (r >> 2)) & 3));
+            }
+            so[i] = (uint32_t)(o + (WIN ? 0 : r * KVD * 2));
+            kr[i] = r;
+            dl[i] = lds0 + (uint32_t)(1024 * u) + (i == 8 ? TL_OK : r0 ? 0 : TL_O1);
+        }
+        auto load = [&](int i, int t, uint32_t d) {
+            uint32_t o;
+            if (WIN) {
+                const int v = 32 * t + kr[i];          /* past the chunk: out of range */
+                o = v < j.nk ? (uint32_t)tl_key(a, j, j.v0 + v) * (KVD * 2) + so[i] : 0xFFFFF000u;
+            } else {
+                o = so[i] + (uint32_t)t * (32 * KVD * 2);
+            }
+            lds_dma16_buf(o, rk, dl[i] + d);
+        };
+        /* latents 0..287 of a tile; 288..575 */
+        auto issue0 = [&](int t) {
+            const uint32_t d = (uint32_t)(t & 3) * TL_R0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) load(i, t, d);
+            if (bw < 2) load(4, t, d);
+        };
+        auto issue1 = [&](int t) {
+            const uint32_t d = (uint32_t)(t % 3) * TL_R1;
+            if (bw >= 2) load(4, t, d);
+#pragma unroll
+            for (int i = 5; i < 8; i++) load(i, t, d);
+            load(8, t, (uint32_t)(t & 1) * TL_KP);
+        };
+        if (nt > 0) issue0(0);
+        if (nt > 1) issue0(1);
+        if (nt > 0) issue1(0);
+        if (nt > 2) issue0(2);
+        if (nt > 1) issue1(1);
+
+        /* transposing reads: lane i of 16-lane group g supplies row 4 (4 s + 2 e
+         * + g / 2) + i / 4, 4 columns from 16 (g % 2) + 4 (i % 4) of column tile ct */
+        const int i16 = lane & 15, gq = lane >> 4, h = gq >> 1;
+        uint32_t va[4][2][2];                          /* [ct][s][e], without the tile's place */
+#pragma unroll
+        for (int ct = 0; ct < 4; ct++)
+#pragma unroll
+            for (int s = 0; s < 2; s++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int col4 = 4 * bw + ct;      /* 32-column tile of the 16 */
+                    const bool r0 = col4 < 9;
+                    const int r = 16 * s + 8 * e + 4 * h + (i16 >> 2);
+                    const int low = (2 * (gq & 1) + ((i16 >> 1) & 1)) ^ (2 * e + h);
+                    va[ct][s][e] = lds0 + (r0 ? 0 : TL_O1) + (uint32_t)(r * (r0 ? 576 : 448) + 64 * (r0 ? col4 : col4 - 9) + 16 * low + 8 * (i16 & 1));
+                }
+        const uint32_t pa = lds0 + TL_OP + (uint32_t)(c32 * 64 + 16 * (hi ^ ((c32 >> 2) & 3)));   /* piece 2 s + hi: s flips bit 1 */
+        auto run = [&](auto rtc) {
+            constexpr int RT = decltype(rtc)::value;   /* row tiles */
+            f32x16 O[RT][4] = {};
+            for (int t = 0; t < nt; t++) {
+                if (t + 3 < nt) issue0(t + 3);
+                if (t + 2 < nt) issue1(t + 2);
+                const uint32_t d0 = (uint32_t)(t & 3) * TL_R0, d1 = (uint32_t)(t % 3) * TL_R1;
+                const uint32_t po = (uint32_t)(t & 1) * 8192;
+                const i32x4 flags = *(lds_w4)(uintptr_t)(lds0 + TL_OG + 16 * (t & 1));
+                if (WIN) {
+                    /* a key that is not finite meets probabilities of zero (rows
+                     * that do not see it; those that do have no finite sum): its
+                     * values, of which this wave alone reads these columns, are
+                     * zeroed */
+                    uint32_t bad = (uint32_t)__builtin_amdgcn_readfirstlane(flags[2] | (RT > 1 ? flags[3] : 0));
+                    while (bad) {
+                        const int r = __builtin_ctz(bad), p = 16 * bw + lane;
+                        bad &= bad - 1;
+                        if (lane < 16) {
+                            const uint32_t o = p < 36 ? d0 + r * 576 + 16 * ((p & ~3) | ((p ^ (r >> 2)) & 3))
+                                                      : TL_O1 + d1 + r * 448 + 16 * (((p - 36) & ~3) | ((p ^ (r >> 2)) & 3));
+                            *(lds_w4)(uintptr_t)(lds0 + o) = (i32x4){0, 0, 0, 0};
+                        }
+                        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    }
+                }
+                i32x4 ph[2][RT], pl[2][RT], v[2][4];
+#pragma unroll
+                for (int s = 0; s < 2; s++) {
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++) {
+                        const uint32_t p = (pa ^ (uint32_t)(32 * s)) + po + 2048 * rt;
+                        ph[s][rt] = *(lds_w4)(uintptr_t)p;
+                        pl[s][rt] = *(lds_w4)(uintptr_t)(p + 4096);
+                    }
+#pragma unroll
+                    for (int ct = 0; ct < 4; ct++) {
+                        const uint32_t d = 4 * bw + ct < 9 ? d0 : d1;
+                        const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(uintptr_t)(va[ct][s][0] + d));
+                        const s16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(uintptr_t)(va[ct][s][1] + d));
+                        v[s][ct] = __builtin_bit_cast(i32x4, (s16x8){x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]});
+                    }
+                }
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) {
+                    if (__builtin_amdgcn_readfirstlane(flags[rt])) {   /* some row's maximum moved: its factor */
+#pragma unroll
+                        for (int g = 0; g < 4; g++) {
+                            const f32x4 f = *(lds_f4)(uintptr_t)(lds0 + TL_OF + (uint32_t)((t & 1) * 256 + 4 * (32 * rt + 8 * g + 4 * hi)));
+#pragma unroll
+                            for (int ct = 0; ct < 4; ct++)
+#pragma unroll
+                                for (int i = 0; i < 4; i++) O[rt][ct][4 * g + i] *= f[i];
+                        }
+                    }
+                }
+#pragma unroll
+                for (int s = 0; s < 2; s++)
+#pragma unroll
+                    for (int ct = 0; ct < 4; ct++)
+#pragma unroll
+                        for (int rt = 0; rt < RT; rt++) {
+                            O[rt][ct] = mfma32(ph[s][rt], v[s][ct], O[rt][ct]);
+                            O[rt][ct] = mfma32(pl[s][rt], v[s][ct], O[rt][ct]);
+                        }
+                VMCNT_WAIT(0);                         /* the loads of this step, a step's products ago */
+                tl_barrier();
+            }
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const i32x4 at = *(lds_w4)(uintptr_t)(lds0 + TL_OT + (uint32_t)(4 * (32 * rt + 8 * g + 4 * hi)));
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        if (32 * rt + 8 * g + 4 * hi + i >= j.nrows) continue;
+                        float *o = a.part_o + (size_t)(uint32_t)at[i] * KVL + 128 * bw + c32;
+#pragma unroll
+                        for (int ct = 0; ct < 4; ct++) o[32 * ct] = O[rt][ct][4 * g + i];
+                    }
+                }
+        };
+        VMCNT_WAIT(0);
+        tl_barrier();                                  /* the first tiles are there */
+        tl_barrier();
+        tl_barrier();
+        if (two) run(std::integral_constant<int, 2>());
+        else run(std::integral_constant<int, 1>());
+        return;
+    }
+
+    /* ---- scores ---- */
+    const int rh = w & 1, second = w >> 1;             /* row half; latents 288.. */
+    if (rh && !two) {
+        for (int t = 0; t < nt + 3; t++) tl_barrier();
+        return;
+    }
+    const int row = j.row0 + min(32 * rh + c32, j.nrows - 1);
+    i32x4 qh[18], ql[18];
+    {
+        const uint16_t *p = a.qhl + (size_t)row * 2 * KVL + 288 * second + 8 * hi;
+#pragma unroll
+        for (int s = 0; s < 14; s++) {
+            qh[s] = *(const i32x4 *)(p + 16 * s);
+            ql[s] = *(const i32x4 *)(p + KVL + 16 * s);
+        }
+        if (second) {
+            const float *qp = a.q + (size_t)row * (a.QKN + MM_MLA_QKR) + a.QKN + 8 * hi;
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                const f32x4 x0 = *(const f32x4 *)(qp + 16 * s), x1 = *(const f32x4 *)(qp + 16 * s + 4);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    uint32_t vh, vl;
+                    split_pk(i < 2 ? x0[2 * i] : x1[2 * i - 4], i < 2 ? x0[2 * i + 1] : x1[2 * i - 3], &vh, &vl);
+                    qh[14 + s][i] = (int)vh;
+                    ql[14 + s][i] = (int)vl;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int s = 14; s < 18; s++) {
+                qh[s] = *(const i32x4 *)(p + 16 * s);
+                ql[s] = *(const i32x4 *)(p + KVL + 16 * s);
+            }
+        }
+    }
+    const int sw = (c32 >> 2) & 3;
+    const uint32_t xa = lds0 + TL_OX + (uint32_t)(rh * 4096 + 16 * lane);
+    tl_barrier();                                      /* the first tiles are there */
+    if (!second) {
+        const uint32_t ka = lds0 + (uint32_t)(c32 * 576);
+        const uint32_t e0 = ka + 16 * (hi ^ sw), e1 = ka + 16 * ((2 + hi) ^ sw);   /* steps 0, 2, ..; 1, 3, .. */
+        for (int t = 0; t < nt; t++) {
+            const uint32_t d = (uint32_t)(t & 3) * TL_R0;
+            f32x16 s1 = {}, s2 = {};
+#pragma unroll
+            for (int s = 0; s < 18; s++) {
+                const i32x4 k = *(lds_w4)(uintptr_t)((s & 1 ? e1 : e0) + d + 64 * (s >> 1));
+                s1 = mfma32(k, qh[s], s1);
+                s2 = mfma32(k, ql[s], s2);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                *(lds_f4)(uintptr_t)(xa + (uint32_t)((t & 1) * 8192 + 1024 * i)) =
+                    (f32x4){s1[4 * i] + s2[4 * i], s1[4 * i + 1] + s2[4 * i + 1], s1[4 * i + 2] + s2[4 * i + 2], s1[4 * i + 3] + s2[4 * i + 3]};
+            tl_barrier();
+        }
+        tl_barrier();
+        tl_barrier();
+        return;
+    }
+    const uint32_t ka = lds0 + TL_O1 + (uint32_t)(c32 * 448), kp = lds0 + TL_OK + (uint32_t)(c32 * 128);
+    const uint32_t e0 = ka + 16 * (hi ^ sw), e1 = ka + 16 * ((2 + hi) ^ sw);
+    uint32_t pe[4];
+#pragma unroll
+    for (int s = 0; s < 4; s++) pe[s] = kp + 16 * ((2 * s + hi) ^ ((c32 >> 1) & 7));
+    const uint32_t pw = lds0 + TL_OP + (uint32_t)((32 * rh + c32) * 64 + 16 * (hi ^ sw));
+    const float scale2 = a.scale * 1.44269504088896341f;   /* scores in units of ln 2 */
+    /* WIN: this lane's position, and those of the block's first and last rows */
+    const int pos = WIN ? j.pos0 + (j.first_row + min(32 * rh + c32, j.nrows - 1)) / a.NH : 0;
+    const int pos_a = WIN ? j.pos0 + j.first_row / a.NH : 0, pos_b = WIN ? j.pos0 + (j.first_row + j.nrows - 1) / a.NH : 0;
+    float m = -INFINITY, l = 0.0f;
+    tl_barrier();
+    for (int t = 0; t < nt; t++) {
+        const uint32_t d = (uint32_t)(t % 3) * TL_R1, dk = (uint32_t)(t & 1) * TL_KP;
+        f32x4 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = *(lds_f4)(uintptr_t)(xa + (uint32_t)((t & 1) * 8192 + 1024 * i));
+        f32x16 s1 = {}, s2 = {};
+#pragma unroll
+        for (int s = 0; s < 18; s++) {
+            const i32x4 k = s < 14 ? *(lds_w4)(uintptr_t)((s & 1 ? e1 : e0) + d + 64 * (s >> 1)) : *(lds_w4)(uintptr_t)(pe[s - 14] + dk);
+            s1 = mfma32(k, qh[s], s1);
+            s2 = mfma32(k, ql[s], s2);
+        }
+        uint32_t bad = 0;
+        bool all = true;                               /* uniform: every row sees every key of the tile */
+        if (WIN) {
+            const int va = j.v0 + 32 * t, vb = va + 31;
+            const int ja = tl_key(a, j, max(va, a.sinks)), jb = tl_key(a, j, vb);
+            all = 32 * t + 31 < j.nk && jb <= pos_a && (jb < a.sinks || ja > pos_b - a.window);
+        } else {
+            all = 32 * t + 31 < j.nk;
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; i++) s1[i] = (s1[i] + s2[i] + x[i >> 2][i & 3]) * scale2;
+        if (!all) {
+            uint32_t own = 0;                          /* this lane's keys that are not finite */
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int v = 32 * t + 8 * (i >> 2) + 4 * hi + (i & 3);
+                bool see = v < j.nk;
+                if (WIN) {
+                    const int key = tl_key(a, j, j.v0 + v);
+                    const bool nf = see && !(fabsf(s1[i]) < INFINITY);
+                    see = see && key <= pos && (key < a.sinks || key > pos - a.window);
+                    own |= nf ? 1u << (8 * (i >> 2) + 4 * hi + (i & 3)) : 0u;
+                    if (nf) s1[i] = __builtin_nanf("");
+                }
+                if (!see) s1[i] = -INFINITY;
+            }
+            if (WIN && __builtin_amdgcn_ballot_w64(own != 0)) {
+                bad = own;
+#pragma unroll
+                for (int off = 1; off < MM_WAVE; off <<= 1) bad |= (uint32_t)__shfl_xor((int)bad, off, MM_WAVE);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++) mx = fmaxf(mx, s1[i]);
+        const bool moved = __builtin_amdgcn_ballot_w64(mx > m + XTAU) != 0;
+        if (moved) {                                   /* lazy rescaling, as in mm_mla_attn */
+            mx = fmaxf(mx, __shfl_xor(mx, 32, MM_WAVE));
+            const float mn = fmaxf(m, mx);
+            const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+            l *= f;
+            m = mn;
+            if (hi == 0) ((lds_f)(uintptr_t)(lds0 + TL_OF))[(t & 1) * 64 + 32 * rh + c32] = f;
+        }
+        if (lane == 0) {
+            lds_i fl = (lds_i)(uintptr_t)(lds0 + TL_OG + 16 * (t & 1));
+            fl[rh] = moved ? 1 : 0;
+            if (WIN) fl[2 + rh] = (int)bad;
+        }
+        const float mz = m == -INFINITY ? 0.0f : m;    /* rows with no key yet: probabilities 0 */
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            i32x4 ph, pl;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float p0 = __builtin_amdgcn_exp2f(s1[8 * s + 2 * i] - mz), p1 = __builtin_amdgcn_exp2f(s1[8 * s + 2 * i + 1] - mz);
+                l += p0 + p1;
+                uint32_t vh, vl;
+                split_pk(p0, p1, &vh, &vl);
+                ph[i] = (int)vh;
+                pl[i] = (int)vl;
+            }
+            const uint32_t p = (pw ^ (uint32_t)(32 * s)) + (uint32_t)((t & 1) * 8192);
+            *(lds_w4)(uintptr_t)p = ph;
+            *(lds_w4)(uintptr_t)(p + 4096) = pl;
+        }
+        tl_barrier();
+    }
+    l += __shfl_xor(l, 32, MM_WAVE);
+    if (hi == 0 && 32 * rh + c32 < j.nrows) {
+        const uint32_t at = (uint32_t)((lds_i)(uintptr_t)(lds0 + TL_OT))[32 * rh + c32];
+        a.part_ml[(size_t)(at >> 4) * 32 + (at & 15)] = m * 0.693147180559945309f;
+        a.part_ml[(size_t)(at >> 4) * 32 + 16 + (at & 15)] = l;
+    }
+    tl_barrier();
+}
+
+/* A shared prefix, and one position per sequence over its own keys. */
+extern "C" __global__ __launch_bounds__(512, 2) void mm_mla_attn_tiles(mm_mla_tiles_args a) { tl_block<false>(a); }
+/* Windows with sinks. */
+extern "C" __global__ __launch_bounds__(512, 2) void mm_mla_attn_tiles_w(mm_mla_tiles_args a) { tl_block<true>(a); }
