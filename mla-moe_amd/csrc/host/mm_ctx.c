@@ -102,10 +102,10 @@ static const struct {
     [K_F32_BF16] = {"mm_f32_bf16", MOD_UTIL},
     [K_ROUTER_WIDE] = {"mm_router_wide", MOD_MOE_BF16},
     [K_ROUTE_WIDE] = {"mm_route_wide", MOD_MOE_I8},
-    [K_MLA_ATTN_WINDOW] = {"mm_mla_attn_window", MOD_MLA},
-    [K_MLA_COMBINE_E] = {"mm_mla_combine_e", MOD_MLA},
     [K_MLA_ATTN_TILES] = {"mm_mla_attn_tiles", MOD_MLA},
     [K_MLA_ATTN_TILES_W] = {"mm_mla_attn_tiles_w", MOD_MLA},
+    [K_MLA_MERGE_UV4] = {"mm_mla_merge_uv_4", MOD_MLA},
+    [K_MLA_MERGE_UV8] = {"mm_mla_merge_uv_8", MOD_MLA},
     [K_LOGPROBS] = {"mm_logprobs", MOD_LM_HEAD},
     [K_LOGPROBS_1] = {"mm_logprobs_1", MOD_LM_HEAD},
     [K_LOGPROBS_FINAL] = {"mm_logprobs_final", MOD_LM_HEAD},
@@ -203,11 +203,6 @@ int mm_ctx_create(int device, mm_ctx **out) {
     if (ev && *ev) c->mla_expand_min = atoi(ev);
     ev = getenv("MLAMOE_MLA_PART_MAX");
     if (ev && *ev && atoll(ev) > 0) c->mla_part_max = (size_t)atoll(ev);
-    /* MLAMOE_MLA_TILES_MIN overrides the rows with common keys from which
-     * prefix and window attention takes 64-row tiles */
-    c->mla_tiles_min = MM_MLA_TILES_MIN;
-    ev = getenv("MLAMOE_MLA_TILES_MIN");
-    if (ev && *ev) c->mla_tiles_min = atoi(ev);
     /* MLAMOE_MOE_T_CHUNK lowers the rows of one MoE forward pass (longer
      * calls run in chunks of it; for testing that the chunks agree) */
     c->moe_t_chunk = 0;

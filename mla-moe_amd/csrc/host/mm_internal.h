@@ -79,10 +79,10 @@ typedef enum {
     K_F32_BF16,
     K_ROUTER_WIDE,
     K_ROUTE_WIDE,
-    K_MLA_ATTN_WINDOW,
-    K_MLA_COMBINE_E,
     K_MLA_ATTN_TILES,
     K_MLA_ATTN_TILES_W,
+    K_MLA_MERGE_UV4,
+    K_MLA_MERGE_UV8,
     K_LOGPROBS,
     K_LOGPROBS_1,
     K_LOGPROBS_FINAL,
@@ -155,9 +155,6 @@ struct mm_ctx {
                                    expanded (MLAMOE_MLA_EXPAND_MIN overrides) */
     int mla_rows4;              /* row groups sharing a sequence read its keys once
                                    (MLAMOE_MLA_ROWS4=0: per row, for comparisons) */
-    int mla_tiles_min;          /* rows (positions times heads) with common keys from which
-                                   prefix and window attention takes 64-row tiles
-                                   (MLAMOE_MLA_TILES_MIN overrides) */
     int moe_t_chunk;            /* cap on the rows of one MoE forward pass (0: MM_MOE_T_CHUNK) */
 
     /* growable device workspace */

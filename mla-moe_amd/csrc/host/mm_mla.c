@@ -207,7 +207,7 @@ static int decode_rows(mm_ctx *c, int layer, int B, const float *q, const uint16
     }
     mm_mla_attn_args aa = {qhl, q, cache, kv_lens, kv_len, seq_stride, g->softmax_scale, part_ml,
                            part_o, probs, kv_len, NH, HG, nchunks, QKN, chunk, slots,
-                           direct ? clat : NULL, B, nchunks, 1, 0, 0, 0};
+                           direct ? clat : NULL, B};
     /* dynamic LDS: two 16-key cache tiles per wave (c_kv rows padded to 1056 B,
      * then the k_pe parts); also holds the waves' partial states for the merge */
     const size_t alds = (size_t)MM_MLA_AW * 2 * MM_MLA_TILE_B;   /* two sub-tile stages per wave */

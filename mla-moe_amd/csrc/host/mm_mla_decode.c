@@ -2,9 +2,10 @@
  * side): sequences that share a prefix, and sliding windows with sinks.
  *
  * Both are the chain of mm_mla_absorbed_decode_dev (mm_mla.c) with other keys:
- * absorbed queries, chunk partials (maximum, sum, unnormalised context) per
- * (row, 16 heads, chunk), their merge, W_UV.  A prefix's partials and those of
- * a sequence's own keys stand in one list, so one merge joins them.
+ * absorbed queries, attention in 64-row tiles (mla_tiles.h) that leaves partials
+ * (maximum, sum, unnormalised context) per (row, 16 heads, chunk), their merge,
+ * W_UV.  A prefix's partials and those of a sequence's own keys stand in one
+ * list, so one merge joins them.
  */
 #include "mm_internal.h"
 
@@ -28,28 +29,13 @@ typedef struct {
 /* A call's rows, how their keys are cut, and where its workspace holds what. */
 typedef struct {
     int R, HG;
-    int tiles;                     /* 64 rows per block (mla_tiles.h), else 16 */
     int pchunk, np;                /* the prefix: keys per chunk, chunks */
     int ochunk, no;                /* own keys */
-    int direct;                    /* one chunk of 16-row blocks: they write clat, no merge */
     int G;                         /* rows whose partials are held at once */
-    size_t o_qhl, o_clat, o_ml, o_po, bytes;
+    size_t o_qhl, o_ml, o_po, bytes;
 } decode_plan;
 
-/* Keys per chunk of the 16-row blocks: as decode_rows (mm_mla.c), MM_MLA_CHUNK
- * halved while the grid has fewer than MM_MLA_MIN_BLOCKS blocks and a row at most
- * 64 chunks; doubled where a row would have more than maxch. */
-static int chunk_keys(size_t blocks, int keys, int maxch) {
-    int chunk = MM_MLA_CHUNK;
-    while (chunk > 16 * MM_MLA_AW && blocks * ((keys + chunk - 1) / chunk) < MM_MLA_MIN_BLOCKS &&
-           (keys + chunk / 2 - 1) / (chunk / 2) <= 64)
-        chunk /= 2;
-    if (chunk < MM_MLA_CHUNK && keys > chunk && keys <= chunk + chunk / 2) chunk *= 2;
-    while ((keys + chunk - 1) / chunk > maxch) chunk *= 2;
-    return chunk;
-}
-
-/* Chunks of the 64-row blocks, one block per CU: us of a block with t tiles of 32
+/* The chunks, one block per CU: us of a block with t tiles of 32
  * keys over 64 (or up to 32) rows -- queries, first loads, two tiles until all
  * roles run, its output --, and of the partials written and read back (4 KB per
  * row and chunk at 4 TB/s). */
@@ -95,71 +81,26 @@ static void plan_decode(const mm_ctx *c, int R, const decode_keys *k, decode_pla
     p->R = R;
     p->HG = (NH + 15) / 16;
     p->pchunk = p->np = p->ochunk = p->no = 0;
-    /* rows that meet the same keys */
-    p->tiles = (k->prefix_len > 0 ? (size_t)R * NH : (size_t)k->rows * NH) >= (size_t)c->mla_tiles_min;
+    tiles_chunks(R, NH, k->rows, k->prefix_len, k->own, p);
     int unit = 1;                  /* rows that fill whole tiles */
-    if (p->tiles) {
-        tiles_chunks(R, NH, k->rows, k->prefix_len, k->own, p);
-        while ((unit * NH) % 64) unit++;
-    } else {
-        const int own = k->own < k->sinks + k->window ? k->own : k->sinks + k->window;
-        if (own > 0) p->ochunk = chunk_keys((size_t)R * p->HG, own, MM_MLA_MAXCH / 2);
-        if (own > 0) p->no = (own + p->ochunk - 1) / p->ochunk;
-        if (k->prefix_len > 0) p->pchunk = chunk_keys((size_t)R * p->HG, k->prefix_len, MM_MLA_MAXCH / 2);
-        if (k->prefix_len > 0) p->np = (k->prefix_len + p->pchunk - 1) / p->pchunk;
-    }
-    p->direct = !p->tiles && p->np == 0 && p->no == 1;
-    const size_t row = p->direct ? 0 : (size_t)p->HG * (p->np + p->no) * (16 * MM_MLA_KVL + 32) * 4;
+    while ((unit * NH) % 64) unit++;
+    const size_t row = (size_t)p->HG * (p->np + p->no) * (16 * MM_MLA_KVL + 32) * 4;
     p->G = R;
     if (row && (size_t)R * row > c->mla_part_max) {
         const size_t g = c->mla_part_max / row / unit * unit;
         p->G = g > 0 ? (int)g : unit;
     }
     p->o_qhl = 0;
-    p->o_clat = al256((size_t)R * NH * 2 * MM_MLA_KVL * 2);
-    p->o_ml = p->o_clat + al256((size_t)R * NH * MM_MLA_KVL * 4);
-    const size_t parts = p->direct ? 0 : (size_t)(p->G < R ? p->G : R) * p->HG * (p->np + p->no);
+    p->o_ml = al256((size_t)R * NH * 2 * MM_MLA_KVL * 2);
+    const size_t parts = (size_t)(p->G < R ? p->G : R) * p->HG * (p->np + p->no);
     p->o_po = p->o_ml + al256(parts * 32 * 4);
     p->bytes = p->o_po + al256(parts * 16 * MM_MLA_KVL * 4);
 }
 
-/* Rows r0 .. r0 + n - 1 of the call: their attention partials (or clat). */
-static int attend_16(mm_ctx *c, const decode_plan *p, const decode_keys *k, const uint16_t *qhl, const float *q,
-                     int r0, int n, float *clat, float *ml, float *po) {
-    const mm_mla_config *g = &c->mla;
-    const int NH = g->n_heads, nch = p->np + p->no;
-    const size_t alds = (size_t)MM_MLA_AW * 2 * MM_MLA_TILE_B;
-    int st;
-    mm_mla_attn_args a = {qhl, q, NULL, NULL, 0, 0, g->softmax_scale, ml, po, NULL, 0, NH, p->HG, 0,
-                          g->qk_nope_head_dim, 0, NULL, p->direct ? clat : NULL, n, nch, 1, 0, 0, 0};
-    if (p->np) {                                      /* every row reads sequence 0 */
-        a.cache = k->prefix;
-        a.kv_len = k->prefix_len;
-        a.nchunks = p->np;
-        a.chunk = p->pchunk;
-        const unsigned nt = (unsigned)n * (unsigned)p->HG * (unsigned)p->np;
-        if ((st = mm_launch(c, K_MLA_ATTN, 8 * ((nt + 7) / 8), 1, 1, 64 * MM_MLA_AW, alds, &a))) return st;
-    }
-    if (!p->no) return MM_OK;
-    a.cache = k->cache;
-    a.seq_stride = k->seq_stride;
-    a.kv_lens = k->kv_lens;
-    a.kv_len = k->kv_len;
-    a.nchunks = p->no;
-    a.chunk = p->ochunk;
-    a.rows = k->rows;
-    a.sinks = k->sinks;
-    a.window = k->window;
-    a.row0 = r0;
-    a.part_ml = ml + (size_t)p->np * 32;
-    a.part_o = po + (size_t)p->np * 16 * MM_MLA_KVL;
-    const unsigned nt = (unsigned)n * (unsigned)p->HG * (unsigned)p->no;
-    return mm_launch(c, K_MLA_ATTN_WINDOW, 8 * ((nt + 7) / 8), 1, 1, 64 * MM_MLA_AW, alds, &a);
-}
-
-/* The same in 64-row blocks; the rows are whole sequences, or part of one. */
-static int attend_64(mm_ctx *c, const decode_plan *p, const decode_keys *k, const uint16_t *qhl, const float *q,
-                     int r0, int n, float *ml, float *po) {
+/* Rows r0 .. r0 + n - 1 of the call, whole sequences or part of one: their
+ * partials. */
+static int attend(mm_ctx *c, const decode_plan *p, const decode_keys *k, const uint16_t *qhl, const float *q,
+                  int r0, int n, float *ml, float *po) {
     const mm_mla_config *g = &c->mla;
     const int NH = g->n_heads, M = n * NH, rows = n < k->rows ? n : k->rows, nseq = n / rows;
     mm_mla_tiles_args a = {qhl, q, g->softmax_scale, ml, po, M, NH, p->HG, g->qk_nope_head_dim, p->np + p->no,
@@ -174,41 +115,42 @@ static int attend_64(mm_ctx *c, const decode_plan *p, const decode_keys *k, cons
 static int decode_run(mm_ctx *c, int layer, const decode_plan *p, const float *q, const decode_keys *k,
                       float *ctx_out, char *ws) {
     const mm_mla_config *g = &c->mla;
-    const int NH = g->n_heads, QKN = g->qk_nope_head_dim, R = p->R;
+    const int NH = g->n_heads, QKN = g->qk_nope_head_dim, VHD = g->v_head_dim, R = p->R;
     uint16_t *qhl = (uint16_t *)(ws + p->o_qhl);
-    float *clat = (float *)(ws + p->o_clat), *ml = (float *)(ws + p->o_ml), *po = (float *)(ws + p->o_po);
+    float *ml = (float *)(ws + p->o_ml), *po = (float *)(ws + p->o_po);
     const uint16_t *kv_b = c->mla_kvb[layer];
-    mm_mla_qprep_args qa = {q, kv_b + (size_t)NH * (QKN + g->v_head_dim) * MM_MLA_KVL, NULL, qhl, R, NH, QKN};
+    mm_mla_qprep_args qa = {q, kv_b + (size_t)NH * (QKN + VHD) * MM_MLA_KVL, NULL, qhl, R, NH, QKN};
     const int wide = R >= MM_MLA_WIDE_B;
-    const unsigned rt = (unsigned)((R + 31) / 32);
     int st = mm_launch(c, wide ? K_MLA_QPREP_W : K_MLA_QPREP, MM_MLA_KVL / (wide ? 64 * MM_MLA_WIDE_S : 64),
-                       (unsigned)NH, rt, 256, 0, &qa);
+                       (unsigned)NH, (unsigned)((R + 31) / 32), 256, 0, &qa);
     if (st) return st;
-    mm_mla_combine_args ca = {ml, po, kv_b, NULL, 0, ctx_out, clat, NULL, 0, R, NH, QKN, g->v_head_dim,
-                              p->HG, p->np + p->no, NULL};
     for (int r0 = 0, n; r0 < R; r0 += n) {
         n = R - r0 < p->G ? R - r0 : p->G;
-        if (p->tiles && k->rows > 1 && n < R) {       /* whole sequences, or within one */
+        if (k->rows > 1 && n < R) {                   /* whole sequences, or within one */
             const int left = k->rows - r0 % k->rows;
             if (r0 % k->rows == 0 && n >= k->rows) n = n / k->rows * k->rows;
             else if (n > left) n = left;
         }
         const size_t h0 = (size_t)r0 * NH;
-        const uint16_t *qh = qhl + h0 * 2 * MM_MLA_KVL;
-        const float *qr = q + h0 * (QKN + MM_MLA_QKR);
-        float *cl = clat + h0 * MM_MLA_KVL;
-        st = p->tiles ? attend_64(c, p, k, qh, qr, r0, n, ml, po) : attend_16(c, p, k, qh, qr, r0, n, cl, ml, po);
-        if (st) return st;
-        if (p->direct) continue;
-        mm_mla_combine_args cg = ca;
-        cg.clat = cl;
-        cg.B = n;
-        const unsigned z = (size_t)NH * R < 128 ? MM_MLA_KVL / 128 : 1;
-        if ((st = mm_launch(c, K_MLA_COMBINE_E, (unsigned)NH, (unsigned)n, z, 256, 0, &cg))) return st;
+        if ((st = attend(c, p, k, qhl + h0 * 2 * MM_MLA_KVL, q + h0 * (QKN + MM_MLA_QKR), r0, n, ml, po))) return st;
+        /* blocks of the merge: four waves a position each, a column tile each, for
+         * few positions (4 of 16 heads 7.5 us, with eight waves 10; 16: 8.8, 10.4);
+         * eight waves for more, 4 positions per block as long as every CU has at
+         * most one block, else 8 (64 positions: 10.2, with four waves 11.4; 39 of
+         * 20 heads and 256 columns: 10.6, 11.6); from 256 positions on 16 per block
+         * and a head's columns together (512: 18.3, with eight waves 20.7) */
+        const int ncol = (VHD + 15) / 16, nw = R <= 16 || R >= 256 ? 4 : 8;
+        const int split = R >= 256 ? 1 : (ncol + nw - 1) / nw;
+        int ppb = R >= 256 ? 16 : 4, wpp = 1;
+        if (R > 16 && R < 256 && (size_t)NH * ((R + 3) / 4) * split > 256) ppb = 8;
+        while (2 * wpp * R <= nw) wpp *= 2;
+        const int rt = (n + ppb - 1) / ppb;
+        mm_mla_merge_uv_args ma = {ml, po, kv_b, ctx_out + h0 * VHD, n, NH, p->HG, QKN, VHD, p->np + p->no,
+                                   ppb, split, wpp};
+        const unsigned blocks = (unsigned)NH * (unsigned)rt * (unsigned)split;
+        if ((st = mm_launch(c, nw == 4 ? K_MLA_MERGE_UV4 : K_MLA_MERGE_UV8, blocks, 1, 1, 64 * nw, 0, &ma))) return st;
     }
-    const int vt = wide ? 16 * MM_MLA_WIDE_S : 16;
-    return mm_launch(c, wide ? K_MLA_UV_W : K_MLA_UV, (unsigned)((g->v_head_dim + vt - 1) / vt), (unsigned)NH, rt,
-                     256, 0, &ca);
+    return MM_OK;
 }
 
 /* ---- a prefix that every sequence shares ------------------------------------- */

@@ -480,10 +480,6 @@ typedef struct {
     float *clat;              /* one chunk (nchunks == 1, no probabilities): clat [B, NH, KVL]
                                  written here, O / l as the merge computes it; else 0 */
     int B;
-    int pchunks;              /* chunks per (row, head group) of the partials: nchunks, or more
-                                 where other kernels write some of them */
-    int rows, sinks, window;  /* mm_mla_attn_window: rows per sequence, the keys they see */
-    int row0;                 /* mm_mla_attn_window: block row b is the call's row row0 + b */
 } mm_mla_attn_args;
 
 /* Rows that meet common keys (mla_tiles.h): blocks of 64 rows (position, head)
@@ -492,7 +488,6 @@ typedef struct {
  * where nchunks is 0), then as many for the N = nseq ceil(rows NH / 64)
  * ochunks of the sequences' own keys. */
 #define MM_MLA_TL_LDS 158720      /* dynamic LDS of a block */
-#define MM_MLA_TILES_MIN 1        /* rows from which they are taken */
 typedef struct {
     const uint16_t *qhl;      /* [M, 2, KVL] bf16 */
     const float *q;           /* [M, QKN + QKR] */
@@ -511,6 +506,17 @@ typedef struct {
      * + roff + r */
     int all_rows, roff, sinks, window;
 } mm_mla_tiles_args;
+
+/* Their merge and W_UV product (mm_mla_merge_uv_4, _8: waves per block). */
+typedef struct {
+    const float *part_ml, *part_o;   /* [R, HG, nchunks, ..] */
+    const uint16_t *kv_b;
+    float *ctx;               /* [R, NH * VHD] */
+    int R, NH, HG, QKN, VHD, nchunks;
+    int ppb;                  /* positions per block, at most 16 */
+    int split;                /* blocks over a head's columns, at most ceil(VHD / 16) */
+    int wpp;                  /* waves that share a position: a power of two, wpp R <= waves or 1 */
+} mm_mla_merge_uv_args;
 
 /* Merge the chunk partials, normalise (clat); then ctx = W_UV . clat. */
 typedef struct {

@@ -382,8 +382,7 @@ __device__ __forceinline__ void mla_accumulate(uint32_t t, const float *sv, floa
  *   ([keys][r] row-major) comes from the same LDS rows by transposing reads.
  * The AW waves' partial states merge in LDS into one partial per chunk.
  * Dynamic LDS: AW * 2 * TILE_B bytes (the merge reuses it). */
-template <bool WIN>
-__device__ __forceinline__ void mla_attn(const mm_mla_attn_args &a) {
+extern "C" __global__ __launch_bounds__(AW * MM_WAVE) void mm_mla_attn(mm_mla_attn_args a) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t alds[];
     /* XCD-grouped order for rows of one length; rows of their own lengths
      * (kv_lens) last row first, in index order over the XCDs in turn, so
@@ -397,14 +396,7 @@ __device__ __forceinline__ void mla_attn(const mm_mla_attn_args &a) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, kl = lane & 15;
-    int L = a.kv_lens ? min(a.kv_lens[WIN ? (a.row0 + b) / a.rows : b], a.kv_len) : a.kv_len;
-    int shift = 0;
-    if (WIN) {   /* keys in the order they are met: the sinks, then the window */
-        L = max(L - a.rows + 1 + (a.row0 + b) % a.rows, 0);
-        const int seen = min(L, a.sinks + a.window);
-        shift = L - seen;
-        L = seen;
-    }
+    const int L = a.kv_lens ? min(a.kv_lens[b], a.kv_len) : a.kv_len;
     /* stage st of wave w at (st AW + w) TILE_B: the second stages of all
      * waves are one region, which holds the block's Q before their loads */
     auto stage = [&](int st) { return alds + (size_t)(st * AW + w) * TILE_B; };
@@ -412,7 +404,7 @@ __device__ __forceinline__ void mla_attn(const mm_mla_attn_args &a) {
     const int kpw = a.chunk / AW;                     /* keys per wave */
     const int kbeg = chunk * a.chunk + w * kpw;
     const int kend = min(kbeg + kpw, L);
-    const int seq = WIN ? (a.row0 + b) / a.rows : a.slots ? a.slots[b] : b;
+    const int seq = a.slots ? a.slots[b] : b;
     const uint8_t *cseq = (const uint8_t *)(a.cache + (size_t)seq * a.seq_stride * KVD);
     /* sub-tile at key k0 -> stage st: row p's c_kv (1 KB, one load per lane
      * of 16 B) at p * CROW_B; the k_pe parts (128 B per row) of rows 0..7 and
@@ -424,14 +416,12 @@ __device__ __forceinline__ void mla_attn(const mm_mla_attn_args &a) {
         uint8_t *t = stage(st);
 #pragma unroll
         for (int p = 0; p < 16; p++) {
-            int key = __builtin_amdgcn_readfirstlane(min(k0 + p, klast));
-            if (WIN) key += key >= a.sinks ? shift : 0;
+            const int key = __builtin_amdgcn_readfirstlane(min(k0 + p, klast));
             lds_dma16(cseq + (uint32_t)(key * KVD * 2) + lane * 16, t + p * CROW_B);
         }
 #pragma unroll
         for (int p = 0; p < 2; p++) {
-            int key = min(k0 + 8 * p + (lane >> 3), klast);
-            if (WIN) key += key >= a.sinks ? shift : 0;
+            const int key = min(k0 + 8 * p + (lane >> 3), klast);
             lds_dma16(cseq + (uint32_t)(key * KVD * 2 + KVL * 2 + (lane & 7) * 16),
                       t + 16 * CROW_B + p * 1024);
         }
@@ -634,7 +624,7 @@ __device__ __forceinline__ void mla_attn(const mm_mla_attn_args &a) {
             for (int nb = 0; nb < KVL / 16; nb++) o[(4 * g + i) * OROW + nb * 16 + kl] = O[nb][i] * wi;
         }
     }
-    const size_t pidx = ((size_t)(b * a.HG + hg) * a.pchunks + chunk);
+    const size_t pidx = ((size_t)(b * a.HG + hg) * a.nchunks + chunk);
     float *linv = mlb + AW * 32;                     /* [16]: one chunk, 1 / l per head */
     if (w == 0 && g == 0) {
         float lsum = 0.0f;
@@ -644,7 +634,7 @@ __device__ __forceinline__ void mla_attn(const mm_mla_attn_args &a) {
             lsum += mj == -INFINITY ? 0.0f : mlb[j * 32 + 16 + kl] * __expf(mj - mm);
         }
         if (a.clat) {
-            linv[kl] = WIN && lsum == 0.0f ? 0.0f : 1.0f / lsum;   /* a row without a key: zeros */
+            linv[kl] = 1.0f / lsum;
         } else {
             a.part_ml[pidx * 32 + kl] = mm;
             a.part_ml[pidx * 32 + 16 + kl] = lsum;
@@ -675,12 +665,6 @@ __device__ __forceinline__ void mla_attn(const mm_mla_attn_args &a) {
         *(f32x4 *)(po + e) = v;
     }
 }
-
-extern "C" __global__ __launch_bounds__(AW * MM_WAVE) void mm_mla_attn(mm_mla_attn_args a) { mla_attn<false>(a); }
-/* Rows that see the first `sinks` and the last `window` keys up to their own:
- * row r (row0 + b) is position kv_lens[s] - rows + r % rows of sequence s = r /
- * rows. */
-extern "C" __global__ __launch_bounds__(AW * MM_WAVE) void mm_mla_attn_window(mm_mla_attn_args a) { mla_attn<true>(a); }
 
 /* Rows that read one cache sequence in groups of AW (a prefill's
  * consecutive positions): one block per (row group, head group, chunk), a
@@ -891,8 +875,7 @@ extern "C" __global__ __launch_bounds__(AW * MM_WAVE) void mm_mla_attn_rows(mm_m
  * t % (pairs per block) over the chunks of its group t / (pairs per block)
  * (16 loads in flight); with Z > 1 the chunk groups meet in LDS in group
  * order (small batches: more blocks, fewer chunks each). */
-template <bool EMPTY>
-__device__ __forceinline__ void mla_combine(const mm_mla_combine_args &a) {
+extern "C" __global__ __launch_bounds__(256) void mm_mla_combine(mm_mla_combine_args a) {
     __shared__ float wch[MM_MLA_MAXCH];
     __shared__ float stat[2];
     __shared__ float2 red[256];
@@ -922,7 +905,7 @@ __device__ __forceinline__ void mla_combine(const mm_mla_combine_args &a) {
         }
     }
     __syncthreads();
-    const float mx = stat[0], inv = EMPTY && stat[1] == 0.0f ? 0.0f : 1.0f / stat[1];
+    const float mx = stat[0], inv = 1.0f / stat[1];
     static_assert(KVL == 512, "combine: 256 column pairs per sequence and head");
     const int npair = (KVL / 2) / gridDim.z, ng = 256 / npair;   /* pairs per block, chunk groups */
     const int cp = tid % npair, cg = tid / npair;
@@ -957,10 +940,6 @@ __device__ __forceinline__ void mla_combine(const mm_mla_combine_args &a) {
         for (int k = tid; k < L; k += blockDim.x) pr[k] = __expf(pr[k] - mx) * inv;
     }
 }
-
-extern "C" __global__ __launch_bounds__(256) void mm_mla_combine(mm_mla_combine_args a) { mla_combine<false>(a); }
-/* rows without a key: zeros */
-extern "C" __global__ __launch_bounds__(256) void mm_mla_combine_e(mm_mla_combine_args a) { mla_combine<true>(a); }
 
 /* ctx[b, h, v] = sum_r W_UV_h[v, r] clat[b, h, r], a per-head GEMM on bf16
  * MFMA (clat split hi/lo).  grid (ceil(VHD / 16), NH, ceil(B / 32)), 4 waves

@@ -461,3 +461,135 @@ __device__ __forceinline__ void tl_block(const mm_mla_tiles_args &a) {
 extern "C" __global__ __launch_bounds__(512, 2) void mm_mla_attn_tiles(mm_mla_tiles_args a) { tl_block<false>(a); }
 /* Windows with sinks. */
 extern "C" __global__ __launch_bounds__(512, 2) void mm_mla_attn_tiles_w(mm_mla_tiles_args a) { tl_block<true>(a); }
+
+/* The chunks' partials of up to 16 positions of one head merged, and their W_UV
+ * products: ctx = W_UV sum_c e^(m_c - m) O_c / l, the latent contexts meeting the
+ * matrix cores as bf16 pairs from LDS.  One launch and no latent context in memory
+ * between.  A 1-D grid of NH * split * ceil(R / ppb) blocks, heads first (column
+ * splits merge for themselves); NW waves.
+ *
+ * Wave w merges positions w, w + NW, ..; in a call of fewer than NW positions
+ * `wpp` waves share one, each every wpp-th chunk.  Then each takes every NW-th
+ * 16-column tile of the block's columns.  A position without a key: zeros. */
+#define MU_ROW 1040                /* bytes of a position's 512 latents in LDS, and 16 */
+template <int NW>
+__device__ __forceinline__ void merge_uv(const mm_mla_merge_uv_args &a) {
+    __shared__ __attribute__((aligned(16))) uint8_t mlds[2 * 16 * MU_ROW];
+    __shared__ f32x4 red[NW - 1][2][MM_WAVE];
+    const int id = (int)blockIdx.x, h = id % a.NH, sp = id / a.NH % a.split, b0 = id / (a.NH * a.split) * a.ppb;
+    const int lane = threadIdx.x & (MM_WAVE - 1);
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / MM_WAVE);
+    const int nrows = min(a.ppb, a.R - b0);
+    const int G = a.wpp;                               /* waves per position */
+    const int cg = w % G;
+    const int ncol = (a.VHD + 15) / 16, per = (ncol + a.split - 1) / a.split;
+    const int ct0 = sp * per, ct1 = min(ct0 + per, ncol);
+    const int n16 = lane & 15, kq = 8 * (lane >> 4);
+    typedef const __attribute__((address_space(1))) i32x4 *glb_c4;
+    const uint16_t *wuv = a.kv_b + ((size_t)h * (a.QKN + a.VHD) + a.QKN) * KVL;
+    /* this wave's first column tile's weights: in flight during the merge */
+    i32x4 wv[KVL / 32];
+    auto weights = [&](int ct) {
+        const uint16_t *p = wuv + (size_t)min(16 * ct + n16, a.VHD - 1) * KVL + kq;
+#pragma unroll
+        for (int s = 0; s < KVL / 32; s++) wv[s] = *(glb_c4)(uintptr_t)(p + 32 * s);
+    };
+    weights(min(ct0 + w, ncol - 1));
+
+    /* the first 64 chunks' maxima and sums of this wave's positions, all in flight
+     * together: lane c has chunk c */
+    float mcs[16 / NW], lcs[16 / NW];
+#pragma unroll
+    for (int i = 0; i < 16 / NW; i++) {
+        const size_t pb = ((size_t)(b0 + min(w / G + i * (NW / G), nrows - 1)) * a.HG + (h >> 4)) * a.nchunks;
+        const float *ml = a.part_ml + (pb + min(lane, a.nchunks - 1)) * 32 + (h & 15);
+        mcs[i] = ml[0];
+        lcs[i] = ml[16];
+    }
+#pragma unroll
+    for (int ri = 0; ri < 16 / NW; ri++) {
+        const int r = w / G + ri * (NW / G);
+        if (r >= nrows) break;
+        const size_t pb = ((size_t)(b0 + r) * a.HG + (h >> 4)) * a.nchunks;
+        const float *ml = a.part_ml + pb * 32 + (h & 15);
+        const float *po = a.part_o + (pb * 16 + (h & 15)) * KVL + 4 * lane;
+        float mx = mcs[ri];                            /* lanes past the chunks hold the last one's */
+        for (int c = MM_WAVE + lane; c < a.nchunks; c += MM_WAVE) mx = fmaxf(mx, ml[(size_t)c * 32]);
+        mx = wave_max(mx);
+        float l = 0.0f;
+        f32x4 s0 = {0.0f, 0.0f, 0.0f, 0.0f}, s1 = s0;
+        for (int cb = 0; cb < a.nchunks; cb += MM_WAVE) {
+            const int cl = min(cb + lane, a.nchunks - 1);
+            const float mc = cb ? ml[(size_t)cl * 32] : mcs[ri], lc = cb ? ml[(size_t)cl * 32 + 16] : lcs[ri];
+            const float wc = cb + lane < a.nchunks && mc != -INFINITY ? __expf(mc - mx) : 0.0f;
+            l += lc * wc;
+            const int n = min(MM_WAVE, a.nchunks - cb);
+            constexpr int U = 8;                       /* chunks whose loads are in flight */
+            for (int c0 = cg; c0 < n; c0 += U * G) {
+                f32x4 v[U][2];
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const float *p = po + (size_t)(cb + min(c0 + u * G, n - 1)) * 16 * KVL;
+                    v[u][0] = *(const f32x4 *)p;
+                    v[u][1] = *(const f32x4 *)(p + 256);
+                }
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int c = c0 + u * G;
+                    if (c >= n) break;                 /* uniform */
+                    const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wc), c));
+                    s0 += v[u][0] * f;
+                    s1 += v[u][1] * f;
+                }
+            }
+        }
+        l = wave_sum(l);
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        if (G > 1) {
+            /* one position per group of G waves: their sums meet in its first */
+            if (cg > 0) {
+                red[w - 1][0][lane] = s0;
+                red[w - 1][1][lane] = s1;
+            }
+            __syncthreads();
+            if (cg == 0)
+                for (int u = 1; u < G; u++) {
+                    s0 += red[w + u - 1][0][lane];
+                    s1 += red[w + u - 1][1][lane];
+                }
+        }
+        if (cg == 0) {
+            typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                const f32x4 s = q ? s1 * inv : s0 * inv;
+                uint32_t h0, h1, l0, l1;
+                split_pk(s[0], s[1], &h0, &l0);
+                split_pk(s[2], s[3], &h1, &l1);
+                *(u32x2 *)(mlds + r * MU_ROW + 512 * q + 8 * lane) = (u32x2){h0, h1};
+                *(u32x2 *)(mlds + (16 + r) * MU_ROW + 512 * q + 8 * lane) = (u32x2){l0, l1};
+            }
+        }
+    }
+    __syncthreads();
+    const int ra = min(n16, nrows - 1) * MU_ROW + 2 * kq;
+    for (int ct = ct0 + w; ct < ct1; ct += NW) {
+        if (ct != ct0 + w) weights(ct);
+        f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f}, yl = y;
+#pragma unroll
+        for (int s = 0; s < KVL / 32; s++) {
+            const i32x4 xh = *(const i32x4 *)(mlds + ra + 64 * s), xl = *(const i32x4 *)(mlds + 16 * MU_ROW + ra + 64 * s);
+            y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, xh), __builtin_bit_cast(bf16x8, wv[s]), y, 0, 0, 0);
+            yl = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, xl), __builtin_bit_cast(bf16x8, wv[s]), yl, 0, 0, 0);
+        }
+        const int v = 16 * ct + n16;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = 4 * (lane >> 4) + i;
+            if (r < nrows && v < a.VHD) a.ctx[((size_t)(b0 + r) * a.NH + h) * a.VHD + v] = y[i] + yl[i];
+        }
+    }
+}
+
+extern "C" __global__ __launch_bounds__(256) void mm_mla_merge_uv_4(mm_mla_merge_uv_args a) { merge_uv<4>(a); }
+extern "C" __global__ __launch_bounds__(512) void mm_mla_merge_uv_8(mm_mla_merge_uv_args a) { merge_uv<8>(a); }
