@@ -79,6 +79,9 @@ typedef enum {
     K_F32_BF16,
     K_ROUTER_WIDE,
     K_ROUTE_WIDE,
+    K_MLA_QFRAG,
+    K_MLA_QFRAG_8,
+    K_MLA_QFRAG_W,
     K_MLA_ATTN_TILES,
     K_MLA_ATTN_TILES_W,
     K_MLA_MERGE_UV4,

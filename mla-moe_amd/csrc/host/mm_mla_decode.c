@@ -32,7 +32,7 @@ typedef struct {
     int pchunk, np;                /* the prefix: keys per chunk, chunks */
     int ochunk, no;                /* own keys */
     int G;                         /* rows whose partials are held at once */
-    size_t o_qhl, o_ml, o_po, bytes;
+    size_t o_ml, o_po, bytes;      /* (the queries at 0) */
 } decode_plan;
 
 /* The chunks, one block per CU: us of a block with t tiles of 32
@@ -90,8 +90,7 @@ static void plan_decode(const mm_ctx *c, int R, const decode_keys *k, decode_pla
         const size_t g = c->mla_part_max / row / unit * unit;
         p->G = g > 0 ? (int)g : unit;
     }
-    p->o_qhl = 0;
-    p->o_ml = al256((size_t)R * NH * 2 * MM_MLA_KVL * 2);
+    p->o_ml = ((size_t)R * NH + 31) / 32 * MM_MLA_QF_TILE;
     const size_t parts = (size_t)(p->G < R ? p->G : R) * p->HG * (p->np + p->no);
     p->o_po = p->o_ml + al256(parts * 32 * 4);
     p->bytes = p->o_po + al256(parts * 16 * MM_MLA_KVL * 4);
@@ -99,11 +98,11 @@ static void plan_decode(const mm_ctx *c, int R, const decode_keys *k, decode_pla
 
 /* Rows r0 .. r0 + n - 1 of the call, whole sequences or part of one: their
  * partials. */
-static int attend(mm_ctx *c, const decode_plan *p, const decode_keys *k, const uint16_t *qhl, const float *q,
-                  int r0, int n, float *ml, float *po) {
+static int attend(mm_ctx *c, const decode_plan *p, const decode_keys *k, const uint16_t *qf, int r0, int n,
+                  float *ml, float *po) {
     const mm_mla_config *g = &c->mla;
     const int NH = g->n_heads, M = n * NH, rows = n < k->rows ? n : k->rows, nseq = n / rows;
-    mm_mla_tiles_args a = {qhl, q, g->softmax_scale, ml, po, M, NH, p->HG, g->qk_nope_head_dim, p->np + p->no,
+    mm_mla_tiles_args a = {qf, r0 * NH, g->softmax_scale, ml, po, M, NH, p->HG, p->np + p->no,
                            k->prefix, k->prefix_len, p->pchunk, p->np, k->cache, k->kv_lens, k->kv_len, k->seq_stride,
                            r0 / k->rows, nseq, rows, p->ochunk, p->no, k->rows, r0 % k->rows, k->sinks, k->window};
     const unsigned np = (unsigned)((M + 63) / 64) * (unsigned)p->np;
@@ -116,13 +115,19 @@ static int decode_run(mm_ctx *c, int layer, const decode_plan *p, const float *q
                       float *ctx_out, char *ws) {
     const mm_mla_config *g = &c->mla;
     const int NH = g->n_heads, QKN = g->qk_nope_head_dim, VHD = g->v_head_dim, R = p->R;
-    uint16_t *qhl = (uint16_t *)(ws + p->o_qhl);
+    uint16_t *qf = (uint16_t *)ws;
     float *ml = (float *)(ws + p->o_ml), *po = (float *)(ws + p->o_po);
     const uint16_t *kv_b = c->mla_kvb[layer];
-    mm_mla_qprep_args qa = {q, kv_b + (size_t)NH * (QKN + VHD) * MM_MLA_KVL, NULL, qhl, R, NH, QKN};
-    const int wide = R >= MM_MLA_WIDE_B;
-    int st = mm_launch(c, wide ? K_MLA_QPREP_W : K_MLA_QPREP, MM_MLA_KVL / (wide ? 64 * MM_MLA_WIDE_S : 64),
-                       (unsigned)NH, (unsigned)((R + 31) / 32), 256, 0, &qa);
+    mm_mla_qfrag_args qa = {q, kv_b + (size_t)NH * (QKN + VHD) * MM_MLA_KVL, qf, R, NH, QKN};
+    const unsigned hg8 = (unsigned)(NH + 7) / 8;
+    int st;
+    if (R < 48)
+        st = mm_launch(c, K_MLA_QFRAG, MM_MLA_KVL / 64 + 1, (unsigned)NH, (unsigned)(R + 31) / 32, 256, 0, &qa);
+    else if (R < 256)
+        st = mm_launch(c, K_MLA_QFRAG_8, MM_MLA_KVL / 32 + 1, hg8, (unsigned)(R + 15) / 16, 512, 0, &qa);
+    else
+        st = mm_launch(c, K_MLA_QFRAG_W, MM_MLA_KVL / (32 * MM_MLA_QF_S) + 1, hg8,
+                       (unsigned)(R + 16 * MM_MLA_QF_NX - 1) / (16 * MM_MLA_QF_NX), 512, 0, &qa);
     if (st) return st;
     for (int r0 = 0, n; r0 < R; r0 += n) {
         n = R - r0 < p->G ? R - r0 : p->G;
@@ -132,7 +137,7 @@ static int decode_run(mm_ctx *c, int layer, const decode_plan *p, const float *q
             else if (n > left) n = left;
         }
         const size_t h0 = (size_t)r0 * NH;
-        if ((st = attend(c, p, k, qhl + h0 * 2 * MM_MLA_KVL, q + h0 * (QKN + MM_MLA_QKR), r0, n, ml, po))) return st;
+        if ((st = attend(c, p, k, qf, r0, n, ml, po))) return st;
         /* blocks of the merge: four waves a position each, a column tile each, for
          * few positions (4 of 16 heads 7.5 us, with eight waves 10; 16: 8.8, 10.4);
          * eight waves for more, 4 positions per block as long as every CU has at

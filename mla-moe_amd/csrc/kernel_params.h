@@ -488,13 +488,24 @@ typedef struct {
  * where nchunks is 0), then as many for the N = nseq ceil(rows NH / 64)
  * ochunks of the sequences' own keys. */
 #define MM_MLA_TL_LDS 158720      /* dynamic LDS of a block */
+#ifndef MM_MLA_QF_NX
+#define MM_MLA_QF_NX 2            /* mm_mla_qfrag_w: 16-position and 32-latent tiles per wave */
+#define MM_MLA_QF_S 4
+#endif
+#define MM_MLA_QF_TILE (2 * 72 * 512)   /* bytes of 32 rows' queries: hi and lo, 72 pieces of 8 latents */
 typedef struct {
-    const uint16_t *qhl;      /* [M, 2, KVL] bf16 */
-    const float *q;           /* [M, QKN + QKR] */
+    const float *q;           /* [R, NH, QKN + QKR] */
+    const uint16_t *wukT;     /* [NH, KVL, QKN] */
+    uint16_t *qf;             /* [ceil(R NH / 32)] tiles of MM_MLA_QF_TILE bytes */
+    int R, NH, QKN;
+} mm_mla_qfrag_args;
+typedef struct {
+    const uint16_t *qf;       /* the call's queries (mm_mla_qfrag) */
+    int row0;                 /* the launch's first row among them */
     float scale;
     float *part_ml;           /* [M / NH, HG, pchunks, 2, 16] */
     float *part_o;            /* [M / NH, HG, pchunks, 16, KVL] */
-    int M, NH, HG, QKN, pchunks;
+    int M, NH, HG, pchunks;
     const uint16_t *keys;     /* [nkeys, KVD] bf16: the prefix */
     int nkeys, chunk, nchunks;   /* keys per block: a multiple of 32 */
     const uint16_t *cache;    /* [sequences, seq_stride, KVD] bf16 */

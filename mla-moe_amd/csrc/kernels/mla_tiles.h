@@ -181,7 +181,7 @@ __device__ __forceinline__ void tl_block(const mm_mla_tiles_args &a) {
             for (int i = 5; i < 8; i++) load(i, t, d);
             load(8, t, (uint32_t)(t & 1) * TL_KP);
         };
-        if (nt > 0) issue0(0);
+        if (nt > 0) issue0(0);                         /* 4 or 5 loads; with issue1 9 in all */
         if (nt > 1) issue0(1);
         if (nt > 0) issue1(0);
         if (nt > 2) issue0(2);
@@ -286,9 +286,25 @@ __device__ __forceinline__ void tl_block(const mm_mla_tiles_args &a) {
                     }
                 }
         };
-        VMCNT_WAIT(0);
-        tl_barrier();                                  /* the first tiles are there */
+        /* the first barrier: issue0(0) done; the next: issue0(1) and issue1(0);
+         * then all */
+        if (nt > 2) {
+            VMCNT_WAIT(18);
+        } else if (nt == 2) {
+            VMCNT_WAIT(9);
+        } else {
+            VMCNT_WAIT(4);
+        }
         tl_barrier();
+        if (nt > 2) {
+            VMCNT_WAIT(9);
+        } else if (nt == 2) {
+            VMCNT_WAIT(4);
+        } else {
+            VMCNT_WAIT(0);
+        }
+        tl_barrier();
+        VMCNT_WAIT(0);
         tl_barrier();
         if (two) run(std::integral_constant<int, 2>());
         else run(std::integral_constant<int, 1>());
@@ -301,39 +317,19 @@ __device__ __forceinline__ void tl_block(const mm_mla_tiles_args &a) {
         for (int t = 0; t < nt + 3; t++) tl_barrier();
         return;
     }
-    const int row = j.row0 + min(32 * rh + c32, j.nrows - 1);
     i32x4 qh[18], ql[18];
     {
-        const uint16_t *p = a.qhl + (size_t)row * 2 * KVL + 288 * second + 8 * hi;
+        const int row = a.row0 + j.row0 + min(32 * rh + c32, j.nrows - 1);
+        const uint8_t *p = (const uint8_t *)a.qf + (size_t)(row >> 5) * MM_MLA_QF_TILE + (36 * second + hi) * 512 + 16 * (row & 31);
 #pragma unroll
-        for (int s = 0; s < 14; s++) {
-            qh[s] = *(const i32x4 *)(p + 16 * s);
-            ql[s] = *(const i32x4 *)(p + KVL + 16 * s);
-        }
-        if (second) {
-            const float *qp = a.q + (size_t)row * (a.QKN + MM_MLA_QKR) + a.QKN + 8 * hi;
-#pragma unroll
-            for (int s = 0; s < 4; s++) {
-                const f32x4 x0 = *(const f32x4 *)(qp + 16 * s), x1 = *(const f32x4 *)(qp + 16 * s + 4);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    uint32_t vh, vl;
-                    split_pk(i < 2 ? x0[2 * i] : x1[2 * i - 4], i < 2 ? x0[2 * i + 1] : x1[2 * i - 3], &vh, &vl);
-                    qh[14 + s][i] = (int)vh;
-                    ql[14 + s][i] = (int)vl;
-                }
-            }
-        } else {
-#pragma unroll
-            for (int s = 14; s < 18; s++) {
-                qh[s] = *(const i32x4 *)(p + 16 * s);
-                ql[s] = *(const i32x4 *)(p + KVL + 16 * s);
-            }
+        for (int s = 0; s < 18; s++) {
+            qh[s] = *(const i32x4 *)(p + 1024 * s);
+            ql[s] = *(const i32x4 *)(p + MM_MLA_QF_TILE / 2 + 1024 * s);
         }
     }
     const int sw = (c32 >> 2) & 3;
     const uint32_t xa = lds0 + TL_OX + (uint32_t)(rh * 4096 + 16 * lane);
-    tl_barrier();                                      /* the first tiles are there */
+    tl_barrier();                                      /* the first tile's latents 0..287 are there */
     if (!second) {
         const uint32_t ka = lds0 + (uint32_t)(c32 * 576);
         const uint32_t e0 = ka + 16 * (hi ^ sw), e1 = ka + 16 * ((2 + hi) ^ sw);   /* steps 0, 2, ..; 1, 3, .. */
@@ -456,6 +452,153 @@ __device__ __forceinline__ void tl_block(const mm_mla_tiles_args &a) {
     }
     tl_barrier();
 }
+
+/* Absorbed queries and q_pe as the score waves read them: bf16 pairs in 32-row
+ * tiles [hi, lo][72 pieces of 8 latents][32 rows][16 bytes], so that a wave's load
+ * is 1 KB.  (From row-major planes each load met 32 lines, 2 us per block.)
+ *
+ * W_UK comes first, as two 16-row tiles whose rows are latents 8 g + i and 8 g +
+ * 4 + i (row 4 g + i), so that a lane ends with the 8 latents of a piece. */
+__device__ __forceinline__ void qf_split(const f32x4 &x0, const f32x4 &x1, i32x4 &ph, i32x4 &pl) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t vh, vl;
+        split_pk(i < 2 ? x0[2 * i] : x1[2 * i - 4], i < 2 ? x0[2 * i + 1] : x1[2 * i - 3], &vh, &vl);
+        ph[i] = (int)vh;
+        pl[i] = (int)vl;
+    }
+}
+__device__ __forceinline__ uint8_t *qf_place(const mm_mla_qfrag_args &a, int b, int h, int piece) {
+    const size_t r = (size_t)b * a.NH + h;
+    return (uint8_t *)a.qf + (r >> 5) * MM_MLA_QF_TILE + 512 * piece + 16 * (r & 31);
+}
+/* One wave: latents e0 .. e0 + 32 S - 1 of head h for NX x 16 positions (b[x]:
+ * lane % 16's of the x-th); ph / pl[s][x] piece e0 / 8 + 4 s + lane / 16. */
+template <int NX, int S>
+__device__ __forceinline__ void qf_wave(const mm_mla_qfrag_args &a, int h, const int (&b)[NX], int e0, i32x4 (&ph)[S][NX], i32x4 (&pl)[S][NX]) {
+    const int lane = threadIdx.x & 63, n16 = lane & 15, g = lane >> 4;
+    const uint16_t *wr = a.wukT + ((size_t)h * KVL + e0 + 8 * (n16 >> 2) + (n16 & 3)) * a.QKN + 8 * g;
+    const float *qr[NX];
+#pragma unroll
+    for (int x = 0; x < NX; x++) qr[x] = a.q + ((size_t)b[x] * a.NH + h) * (a.QKN + MM_MLA_QKR) + 8 * g;
+    f32x4 y[S][NX][2] = {};
+    constexpr int GB = S * NX > 2 ? 2 : 4;             /* 32-wide steps whose loads are in flight */
+    for (int k0 = 0; k0 < a.QKN; k0 += 32 * GB) {
+        i32x4 wv[GB][S][2];
+        f32x4 xv[GB][NX][2];
+#pragma unroll
+        for (int u = 0; u < GB; u++) {
+            const int k = min(k0 + 32 * u, a.QKN - 32);
+#pragma unroll
+            for (int s = 0; s < S; s++) {
+                wv[u][s][0] = *(const i32x4 *)(wr + 32 * s * a.QKN + k);
+                wv[u][s][1] = *(const i32x4 *)(wr + (32 * s + 4) * a.QKN + k);
+            }
+#pragma unroll
+            for (int x = 0; x < NX; x++) {
+                xv[u][x][0] = *(const f32x4 *)(qr[x] + k);
+                xv[u][x][1] = *(const f32x4 *)(qr[x] + k + 4);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);             /* (the loads sink to their uses otherwise, one at a time) */
+#pragma unroll
+        for (int u = 0; u < GB; u++) {
+            if (k0 + 32 * u >= a.QKN) break;
+#pragma unroll
+            for (int x = 0; x < NX; x++) {
+                i32x4 xh, xl;
+                qf_split(xv[u][x][0], xv[u][x][1], xh, xl);
+#pragma unroll
+                for (int s = 0; s < S; s++)
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+                        y[s][x][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wv[u][s][t]), __builtin_bit_cast(bf16x8, xh), y[s][x][t], 0, 0, 0);
+                        y[s][x][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wv[u][s][t]), __builtin_bit_cast(bf16x8, xl), y[s][x][t], 0, 0, 0);
+                    }
+            }
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < S; s++)
+#pragma unroll
+        for (int x = 0; x < NX; x++) qf_split(y[s][x][0], y[s][x][1], ph[s][x], pl[s][x]);
+}
+
+/* Few positions: grid (KVL / 64 slabs and one for q_pe, NH, ceil(R / 32)), wave w
+ * latents 32 (w % 2) .. + 31 of the slab for positions 16 (w / 2) .. + 15. */
+extern "C" __global__ __launch_bounds__(256) void mm_mla_qfrag(mm_mla_qfrag_args a) {
+    const int slab = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    i32x4 ph[1][1], pl[1][1];
+    int b, piece;
+    if (slab == KVL / 64) {                            /* q_pe: a piece per thread */
+        b = blockIdx.z * 32 + (tid >> 3);
+        piece = KVL / 8 + (tid & 7);
+        const float *q = a.q + ((size_t)min(b, a.R - 1) * a.NH + h) * (a.QKN + MM_MLA_QKR) + a.QKN + 8 * (tid & 7);
+        qf_split(*(const f32x4 *)q, *(const f32x4 *)(q + 4), ph[0][0], pl[0][0]);
+    } else {
+        const int e0 = 64 * slab + 32 * (w & 1);
+        b = blockIdx.z * 32 + 16 * (w >> 1) + (lane & 15);
+        piece = e0 / 8 + (lane >> 4);
+        const int bc[1] = {min(b, a.R - 1)};
+        qf_wave<1, 1>(a, h, bc, e0, ph, pl);
+    }
+    if (b >= a.R) return;
+    uint8_t *p = qf_place(a, b, h, piece);
+    *(i32x4 *)p = ph[0][0];
+    *(i32x4 *)(p + MM_MLA_QF_TILE / 2) = pl[0][0];
+}
+
+/* More: a block of eight heads (wave w head w), whose 16-byte pieces are one line
+ * and leave together through LDS; 16 NX positions and 32 S latents per wave.  A
+ * wave's reads are 16 rows of 64 bytes each and set the time, so that many
+ * positions take a larger tile (512 of 16 heads, NX x S = 1 x 1 22 us).  grid (KVL
+ * / (32 S) and one for q_pe, ceil(NH / 8), ceil(R / (16 NX))). */
+template <int NX, int S>
+__device__ __forceinline__ void qf_block(const mm_mla_qfrag_args &a) {
+    __shared__ __attribute__((aligned(16))) i32x4 st[2][4][16 * NX][8];   /* [hi, lo][piece][position][head] */
+    const int slab = blockIdx.x, h0 = blockIdx.y * 8, b0 = blockIdx.z * 16 * NX;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int sh = tid & 7, sb = tid >> 3 & 15, sp = tid >> 7;
+    if (slab == KVL / (32 * S)) {                      /* q_pe: 8 pieces, 16 NX positions, 8 heads */
+#pragma unroll
+        for (int u = 0; u < 2 * NX; u++) {
+            const int b = b0 + 16 * (u >> 1) + sb, piece = sp + 4 * (u & 1);
+            if (b >= a.R || h0 + sh >= a.NH) continue;
+            const float *q = a.q + ((size_t)b * a.NH + h0 + sh) * (a.QKN + MM_MLA_QKR) + a.QKN + 8 * piece;
+            i32x4 ph, pl;
+            qf_split(*(const f32x4 *)q, *(const f32x4 *)(q + 4), ph, pl);
+            uint8_t *p = qf_place(a, b, h0 + sh, KVL / 8 + piece);
+            *(i32x4 *)p = ph;
+            *(i32x4 *)(p + MM_MLA_QF_TILE / 2) = pl;
+        }
+        return;
+    }
+    i32x4 ph[S][NX], pl[S][NX];
+    int b[NX];
+#pragma unroll
+    for (int x = 0; x < NX; x++) b[x] = min(b0 + 16 * x + (lane & 15), a.R - 1);
+    qf_wave<NX, S>(a, min(h0 + w, a.NH - 1), b, 32 * S * slab, ph, pl);
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+        if (s) __syncthreads();                        /* the pieces before are read */
+#pragma unroll
+        for (int x = 0; x < NX; x++) {
+            st[0][lane >> 4][16 * x + (lane & 15)][w] = ph[s][x];
+            st[1][lane >> 4][16 * x + (lane & 15)][w] = pl[s][x];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < NX; x++)
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+                if (b0 + 16 * x + sb < a.R && h0 + sh < a.NH)
+                    *(i32x4 *)(qf_place(a, b0 + 16 * x + sb, h0 + sh, 4 * (S * slab + s) + sp) + u * (MM_MLA_QF_TILE / 2)) = st[u][sp][16 * x + sb][sh];
+    }
+}
+extern "C" __global__ __launch_bounds__(512) void mm_mla_qfrag_8(mm_mla_qfrag_args a) { qf_block<1, 1>(a); }
+extern "C" __global__ __launch_bounds__(512) void mm_mla_qfrag_w(mm_mla_qfrag_args a) { qf_block<MM_MLA_QF_NX, MM_MLA_QF_S>(a); }
 
 /* A shared prefix, and one position per sequence over its own keys. */
 extern "C" __global__ __launch_bounds__(512, 2) void mm_mla_attn_tiles(mm_mla_tiles_args a) { tl_block<false>(a); }
