@@ -67,7 +67,7 @@ int mm_token_logprobs_workspace(int T, int n, int n_top, size_t *bytes) {
     int st = logprobs_check(T, n, n_top), nseg;
     if (st || T == 0) return st;
     logprobs_seg(T, n, &nseg);
-    if (nseg > 1) *bytes = al256((size_t)T * nseg * 16) + 2 * al256((size_t)T * nseg * n_top * 4);
+    if (nseg > 1) *bytes = al256((size_t)T * nseg * 16) + (size_t)T * nseg * n_top * 8;
     return MM_OK;
 }
 
@@ -88,13 +88,13 @@ int mm_token_logprobs_dev(mm_ctx *c, int T, const float *logits, size_t stride, 
     if ((size_t)T * nseg > 0x7fffffffu)
         return mm_fail(MM_ERR_UNSUPPORTED, "mm_token_logprobs_dev: %d rows of %d", T, n);
     char *p = NULL;
-    const size_t n_s = al256((size_t)T * nseg * 16), n_v = al256((size_t)T * nseg * n_top * 4);
+    const size_t n_s = al256((size_t)T * nseg * 16), n_k = (size_t)T * nseg * n_top * 8;
     if (nseg > 1 &&
-        (st = mm_call_workspace(c, "mm_token_logprobs_dev", ws, ws_bytes, n_s + 2 * n_v, (void **)&p)))
+        (st = mm_call_workspace(c, "mm_token_logprobs_dev", ws, ws_bytes, n_s + n_k, (void **)&p)))
         return st;
     mm_logprobs_args a = {logits, stride, targets, logprob, entropy, top_idx, top_logprob,
-                          (float *)p, (float *)(p + n_s), (int32_t *)(p + n_s + n_v), n, n_top, nseg, seg};
-    const int vec = (uintptr_t)logits % 16 == 0 && (T == 1 || stride % 4 == 0) && n >= 4;
+                          (float *)p, (uint64_t *)(p + n_s), n, n_top, nseg, seg};
+    const int vec = (uintptr_t)logits % 16 == 0 && (T == 1 || stride % 4 == 0);
     if ((st = mm_launch(c, vec ? K_LOGPROBS : K_LOGPROBS_1, (unsigned)T * (unsigned)nseg, 1, 1, 256, 0, &a)))
         return st;
     return nseg > 1 ? mm_launch(c, K_LOGPROBS_FINAL, (unsigned)T, 1, 1, 64, 0, &a) : MM_OK;

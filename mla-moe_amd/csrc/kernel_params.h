@@ -761,8 +761,7 @@ typedef struct {
     int32_t *top_idx;        /* [T, n_top] or 0 */
     float *top_logprob;      /* [T, n_top] or 0 */
     float *part_s;           /* [T, nseg, 4]: m, R, U, list entries (as an int's bits) */
-    float *part_v;           /* [T, nseg, n_top] each segment's largest, sorted */
-    int32_t *part_i;         /* [T, nseg, n_top] their indices */
+    uint64_t *part_k;        /* [T, nseg, n_top] each segment's largest, as keys, sorted */
     int n, n_top, nseg;
     int seg;                 /* elements per segment, a multiple of MM_LP_PASS */
 } mm_logprobs_args;

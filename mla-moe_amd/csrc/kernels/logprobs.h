@@ -12,11 +12,12 @@
  * instructions per element against the ~30 that fit beside the memory's
  * rate).  A wave takes chunks of 1,024 elements of its block's segment, two in
  * flight, every lane with an (m, R, U) of its own; they meet by pairs at the
- * end.  The n_top largest are kept beside: a list in LDS, sorted by (value
- * descending, index ascending), and its last entry as the threshold that an
- * element must beat; a wave meets few such elements after its first chunk,
- * whose threshold is the n_top-th of the lanes' maxima.
- */
+ * end.  The n_top largest are kept beside, as 64-bit keys whose order is (value
+ * descending, index ascending): a list in LDS, compacted by rank, and the key that
+ * an element must beat.  A wave meets few such elements after its first chunk,
+ * which starts from the n_top-th of the lanes' maxima.  All of this is written
+ * once per kernel, in loops: unrolled over a chunk's elements it was instructions
+ * to fetch (one row, 20 alternatives: 13 + 7 us; without any 4 + 2). */
 #define LP_VPL 16                  /* elements per lane and chunk */
 #define LP_CHUNK (LP_VPL * MM_WAVE)
 #define LP_WAVES 4
@@ -38,77 +39,72 @@ __device__ __forceinline__ lp_stat lp_merge(const lp_stat &a, const lp_stat &b) 
     return {mh, Rh + s * w, Uh + w * (Ul + fmaxf(d, LP_DMIN) * s)};
 }
 
-/* (v, i) before (bv, bi): larger, or equal at a lower index */
-__device__ __forceinline__ bool lp_before(float v, int i, float bv, int bi) {
-    return v > bv || (v == bv && i < bi);
+/* Whole numbers in the order of the values (-0 as 0), and back. */
+__device__ __forceinline__ uint32_t lp_ord(float v) {
+    const uint32_t u = __float_as_uint(v + 0.0f);
+    return u ^ (uint32_t)((int32_t)u >> 31 | (int32_t)0x80000000);
 }
+__device__ __forceinline__ float lp_val(uint32_t o) {
+    return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
+}
+#define LP_ORD_NINF 0x007fffffu    /* lp_ord(-inf): nothing that is listed is below */
+__device__ __forceinline__ uint64_t lp_key(float v, int i) { return (uint64_t)lp_ord(v) << 32 | (uint32_t)~i; }
 
-/* A wave's best entries: `cnt` of them in lv / li (LDS, this wave's), and what
- * an element must come before to be one. */
+/* A wave's best entries: `cnt` keys in `l` (LDS, this wave's), and the key that an
+ * element must be above, and its value not below tv, to be one. */
 struct lp_top {
-    float *lv;
-    int *li;
+    uint64_t *l;
     int cnt, k;
+    uint64_t t;
     float tv;
-    int ti;
-    /* the k best of the cnt entries, sorted, to the front: each entry's rank
-     * is the number of entries before it */
+    /* the k best of the cnt entries, sorted, to the front: an entry's rank is
+     * the number of entries above it */
     __device__ __forceinline__ void compact() {
-        const int lane = threadIdx.x & (MM_WAVE - 1);
-        const int n = cnt;
+        const int lane = threadIdx.x & (MM_WAVE - 1), n = cnt;
         asm volatile("" ::: "memory");
-        const float v0 = lv[min(lane, LP_LIST - 1)], v1 = lv[64 + lane];
-        const int i0 = li[lane], i1 = li[64 + lane];
+        const uint64_t k0 = l[lane], k1 = l[64 + lane];
         int r0 = 0, r1 = 0;
-#pragma unroll 4
-        for (int j = 0; j < n; j++) {
-            const float bv = lv[j];
-            const int bi = li[j];
-            r0 += lp_before(bv, bi, v0, i0) ? 1 : 0;
-            r1 += lp_before(bv, bi, v1, i1) ? 1 : 0;
+        for (int j = 0; j < n; j += 8) {
+            uint64_t b[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) b[u] = l[j + u];   /* (n <= LP_LIST, a multiple of 8) */
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const bool in = j + u < n;
+                r0 += in && b[u] > k0 ? 1 : 0;
+                r1 += in && b[u] > k1 ? 1 : 0;
+            }
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        if (lane < n && r0 < k) {
-            lv[r0] = v0;
-            li[r0] = i0;
-        }
-        if (64 + lane < n && r1 < k) {
-            lv[r1] = v1;
-            li[r1] = i1;
-        }
+        if (lane < n && r0 < k) l[r0] = k0;
+        if (64 + lane < n && r1 < k) l[r1] = k1;
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         cnt = min(n, k);
         if (cnt == k) {
-            tv = lv[k - 1];
-            ti = li[k - 1];
+            t = l[k - 1];
+            tv = lp_val((uint32_t)(t >> 32));
         }
     }
-    /* one element per lane; ok: there is one */
-    __device__ __forceinline__ void offer(float v, int i, bool ok) {
-        const bool c = ok && lp_before(v, i, tv, ti);
+    /* one key per lane; ok: there is one */
+    __device__ __forceinline__ void offer(uint64_t key, bool ok) {
+        const bool c = ok && key > t;
         const uint64_t mask = __builtin_amdgcn_ballot_w64(c);
-        if (!mask) return;
         const int at = cnt + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
-        if (c) {
-            lv[at] = v;
-            li[at] = i;
-        }
+        if (c) l[at] = key;
         cnt += __builtin_popcountll(mask);
         if (cnt > 64) compact();
     }
-    /* the k-th largest of the lanes' values (-inf: none): at least k elements
-     * are not below it */
+    /* a value that at least k of the lanes' values (-inf: none) are not below:
+     * the k-th largest, its last 14 bits cleared */
     __device__ __forceinline__ void threshold(float v) {
-        const int lane = threadIdx.x & (MM_WAVE - 1);
-        int r = 0;
-#pragma unroll
-        for (int l = 0; l < MM_WAVE; l++) {
-            const float o = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l));
-            r += lp_before(o, l, v, lane) ? 1 : 0;
-        }
-        const uint64_t at = __builtin_amdgcn_ballot_w64(r == k - 1);
-        tv = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), __builtin_ctzll(at)));
-        ti = 0x7fffffff;
+        const uint32_t o = lp_ord(v);
+        uint32_t p = 0;
+#pragma unroll 1
+        for (uint32_t bit = 0x80000000u; bit >= 1u << 14; bit >>= 1)
+            if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(o >= (p | bit))) >= k) p |= bit;
+        p = max(p, LP_ORD_NINF);
+        t = ((uint64_t)p << 32) - 1;
+        tv = lp_val(p);
     }
 };
 
@@ -143,9 +139,10 @@ __device__ __forceinline__ void lp_finish(const mm_logprobs_args &a, int t, cons
     }
     if (lane < a.n_top) {
         const bool is = lane < top.cnt;
+        const uint64_t key = top.l[lane];
         const size_t o = (size_t)t * a.n_top + lane;
-        if (a.top_idx) a.top_idx[o] = is ? top.li[lane] : -1;
-        if (a.top_logprob) a.top_logprob[o] = is ? (top.lv[lane] - s.m) - lz : __builtin_nanf("");
+        if (a.top_idx) a.top_idx[o] = is ? (int)~(uint32_t)key : -1;
+        if (a.top_logprob) a.top_logprob[o] = is ? (lp_val((uint32_t)(key >> 32)) - s.m) - lz : __builtin_nanf("");
     }
 }
 
@@ -153,8 +150,7 @@ __device__ __forceinline__ void lp_finish(const mm_logprobs_args &a, int t, cons
  * per load (4 where every row is 16-byte aligned). */
 template <int V>
 __device__ __forceinline__ void lp_block(const mm_logprobs_args &a) {
-    __shared__ float lv[LP_WAVES][LP_LIST];
-    __shared__ int li[LP_WAVES][LP_LIST];
+    __shared__ uint64_t ls[LP_WAVES][LP_LIST];
     __shared__ lp_stat ws[LP_WAVES];
     __shared__ int wc[LP_WAVES];
     const int t = (int)(blockIdx.x / (unsigned)a.nseg), seg = (int)(blockIdx.x % (unsigned)a.nseg);
@@ -162,108 +158,94 @@ __device__ __forceinline__ void lp_block(const mm_logprobs_args &a) {
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / MM_WAVE);
     const float *x = a.logits + (size_t)t * a.stride;
     const int n = a.n, s0 = seg * a.seg, s1 = (int)min((int64_t)s0 + a.seg, (int64_t)n);
-    constexpr int NL = LP_VPL / V;
-    typedef float vec __attribute__((ext_vector_type(V == 1 ? 2 : V)));
-    /* element j of this lane in the chunk at c: c + V (64 (j / V) + lane) + j % V.
-     * With V = 4 the loads stop at the row's last whole vector; its up to 3
-     * further elements are offered on their own below. */
-    const int nv = V == 1 ? n : n / V * V;
+    typedef float vec __attribute__((ext_vector_type(4)));
+    /* element j of this lane in the chunk at c is c + at(j); a chunk that the row
+     * ends in is read an element at a time, at clamped indices */
+    auto at = [&](int j) { return V * (MM_WAVE * (j / V) + lane) + j % V; };
     auto load = [&](int c, float (&v)[LP_VPL]) {
+        if (V == 4 && c + LP_CHUNK <= n) {             /* uniform */
 #pragma unroll
-        for (int u = 0; u < NL; u++) {
-            const int i = c + V * (MM_WAVE * u + lane);
-            if (V == 1) {
-                v[u] = x[min(i, n - 1)];
-            } else {
-                const vec d = *(const vec *)(x + min(i, nv - V));
+            for (int u = 0; u < LP_VPL / 4; u++) {
+                const vec d = *(const vec *)(x + c + 4 * (MM_WAVE * u + lane));
 #pragma unroll
-                for (int q = 0; q < V; q++) v[V * u + q] = d[q];
+                for (int q = 0; q < 4; q++) v[4 * u + q] = d[q];
             }
+        } else {
+#pragma unroll
+            for (int j = 0; j < LP_VPL; j++) v[j] = x[min(c + at(j), n - 1)];
         }
     };
     lp_stat st = {-INFINITY, -1.0f, 0.0f};
-    lp_top top = {lv[w], li[w], 0, a.n_top, -INFINITY, 0x7fffffff};
-    const int e1 = min(s1, nv);                       /* chunks cover [s0, e1) */
-    auto take = [&](int c, float (&v)[LP_VPL], bool first) {
-        if (c + LP_CHUNK > e1) {                      /* uniform: the segment's last chunk */
-#pragma unroll
-            for (int j = 0; j < LP_VPL; j++)
-                if (c + V * (MM_WAVE * (j / V) + lane) + j % V >= e1) v[j] = -INFINITY;
-        }
-        float mc = v[0];
-#pragma unroll
-        for (int j = 1; j < LP_VPL; j++) mc = fmaxf(mc, v[j]);
-        mc = fmaxf(mc, -INFINITY);                    /* a lane of NaNs only */
-        lp_add(st, v, mc);
-        if (a.n_top == 0) return;
-        if (first) top.threshold(mc);
-        if (!__builtin_amdgcn_ballot_w64(mc >= top.tv)) return;
-#pragma unroll
-        for (int j = 0; j < LP_VPL; j++) {
-            const int i = c + V * (MM_WAVE * (j / V) + lane) + j % V;
-            if (__builtin_amdgcn_ballot_w64(v[j] >= top.tv)) top.offer(v[j], i, i < e1);
-        }
-    };
+    lp_top top = {ls[w], 0, a.n_top, 0, -INFINITY};
     constexpr int STEP = LP_WAVES * LP_CHUNK;
     const int c0 = s0 + w * LP_CHUNK;
-    if (c0 < e1) {
-        float va[LP_VPL], vb[LP_VPL];
-        load(c0, va);
-        for (int c = c0; c < e1; c += 2 * STEP) {
-            load(c + STEP, vb);                       /* past the end: clamped, not used */
-            take(c, va, c == c0);
-            if (c + STEP >= e1) break;
-            load(c + 2 * STEP, va);
-            take(c + STEP, vb, false);
+    if (c0 < s1) {
+        float v[LP_VPL], nx[LP_VPL];
+        load(c0, v);
+        for (int c = c0;; c += STEP) {
+            const bool more = c + STEP < s1;
+            if (more) load(c + STEP, nx);
+            if (c + LP_CHUNK > s1) {                   /* uniform: the row ends in it */
+#pragma unroll
+                for (int j = 0; j < LP_VPL; j++)
+                    if (c + at(j) >= s1) v[j] = -INFINITY;
+            }
+            float mc = v[0];
+#pragma unroll
+            for (int j = 1; j < LP_VPL; j++) mc = fmaxf(mc, v[j]);
+            mc = fmaxf(mc, -INFINITY);                 /* a lane of NaNs only */
+            lp_add(st, v, mc);
+            if (a.n_top) {
+                if (c == c0) top.threshold(mc);
+                uint32_t cand = 0;                     /* this lane's elements that may be listed */
+#pragma unroll
+                for (int j = 0; j < LP_VPL; j++) cand |= v[j] >= top.tv ? 1u << j : 0u;
+                while (__builtin_amdgcn_ballot_w64(cand != 0)) {
+                    const int j = __builtin_ctz(cand | 1u << (LP_VPL - 1));
+                    float e = v[0];
+#pragma unroll
+                    for (int u = 1; u < LP_VPL; u++) e = j == u ? v[u] : e;
+                    const int i = c + V * (MM_WAVE * (j / V) + lane) + j % V;
+                    top.offer(lp_key(e, i), cand != 0 && i < s1);
+                    cand &= cand - 1;
+                }
+            }
+            if (!more) break;
+#pragma unroll
+            for (int j = 0; j < LP_VPL; j++) v[j] = nx[j];
         }
     }
-    if (V > 1 && nv < n && s1 == n && w == 0) {       /* the row's last n % V elements */
-        const bool ok = lane < n - nv;
-        const float v = ok ? x[min(nv + lane, n - 1)] : -INFINITY;
-        float one[LP_VPL];
-#pragma unroll
-        for (int j = 0; j < LP_VPL; j++) one[j] = j == 0 ? v : -INFINITY;
-        lp_add(st, one, fmaxf(v, -INFINITY));
-        if (a.n_top) top.offer(v, nv + lane, ok);
-    }
-    if (top.cnt) top.compact();
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) {
         const lp_stat o = {__shfl_xor(st.m, off, MM_WAVE), __shfl_xor(st.R, off, MM_WAVE), __shfl_xor(st.U, off, MM_WAVE)};
         st = lp_merge(st, o);
     }
-    if (lane == 0) {
-        ws[w] = st;
-        wc[w] = top.cnt;
-    }
-    __syncthreads();
-    if (w > 0) return;
-    for (int u = 1; u < LP_WAVES; u++) st = lp_merge(st, ws[u]);
-    for (int u = 1; u < LP_WAVES; u++) {              /* the waves' lists, at most LP_LIST entries */
-        const int nu = wc[u];
-        if (lane < nu) {
-            lv[0][top.cnt + lane] = lv[u][lane];
-            li[0][top.cnt + lane] = li[u][lane];
+    /* each wave's list, then (turn 1, wave 0 alone) the waves' lists in one, at
+     * most LP_LIST entries */
+#pragma unroll 1
+    for (int turn = 0; turn < 2; turn++) {
+        if (top.cnt) top.compact();
+        if (turn) break;
+        if (lane == 0) {
+            ws[w] = st;
+            wc[w] = top.cnt;
         }
-        top.cnt += nu;
+        __syncthreads();
+        if (w > 0) return;
+        for (int u = 1; u < LP_WAVES; u++) {
+            st = lp_merge(st, ws[u]);
+            const int nu = wc[u];
+            if (lane < nu) ls[0][top.cnt + lane] = ls[u][lane];
+            top.cnt += nu;
+        }
     }
-    if (top.cnt) top.compact();
     if (a.nseg == 1) {
         lp_finish(a, t, st, top);
         return;
     }
     const size_t p = blockIdx.x;
-    if (lane == 0) {
-        float *ps = a.part_s + 4 * p;
-        ps[0] = st.m;
-        ps[1] = st.R;
-        ps[2] = st.U;
-        ps[3] = __int_as_float(top.cnt);
-    }
-    if (lane < top.cnt) {
-        a.part_v[p * a.n_top + lane] = top.lv[lane];
-        a.part_i[p * a.n_top + lane] = top.li[lane];
-    }
+    if (lane == 0) *(f32x4 *)(a.part_s + 4 * p) = (f32x4){st.m, st.R, st.U, __int_as_float(top.cnt)};
+    if (lane < top.cnt) a.part_k[p * a.n_top + lane] = top.l[lane];
 }
 
 extern "C" __global__ __launch_bounds__(64 * LP_WAVES) void mm_logprobs(mm_logprobs_args a) { lp_block<4>(a); }
@@ -272,11 +254,16 @@ extern "C" __global__ __launch_bounds__(64 * LP_WAVES) void mm_logprobs_1(mm_log
 
 /* One wave per row merges its segments: lane s has segment s. */
 extern "C" __global__ __launch_bounds__(64) void mm_logprobs_final(mm_logprobs_args a) {
-    __shared__ float lv[LP_LIST];
-    __shared__ int li[LP_LIST];
+    __shared__ uint64_t ls[LP_LIST];
     const int t = blockIdx.x, lane = threadIdx.x;
     const size_t p = (size_t)t * a.nseg + min(lane, a.nseg - 1);
     const f32x4 ps = *(const f32x4 *)(a.part_s + 4 * p);
+    const uint64_t *pk = a.part_k + p * a.n_top;
+    constexpr int U = 4;                               /* list entries read together */
+    uint64_t key[U];
+    if (a.n_top)
+#pragma unroll
+        for (int u = 0; u < U; u++) key[u] = pk[min(u, a.n_top - 1)];
     lp_stat st = {ps.x, ps.y, ps.z};
     int have = __float_as_int(ps.w);
     if (lane >= a.nseg) {
@@ -288,17 +275,18 @@ extern "C" __global__ __launch_bounds__(64) void mm_logprobs_final(mm_logprobs_a
         const lp_stat o = {__shfl_xor(st.m, off, MM_WAVE), __shfl_xor(st.R, off, MM_WAVE), __shfl_xor(st.U, off, MM_WAVE)};
         st = lp_merge(st, o);
     }
-    lp_top top = {lv, li, 0, a.n_top, -INFINITY, 0x7fffffff};
+    lp_top top = {ls, 0, a.n_top, 0, -INFINITY};
     if (a.n_top) {
-        const float *pv = a.part_v + p * a.n_top;
-        const int32_t *pi = a.part_i + p * a.n_top;
-        top.threshold(have ? pv[0] : -INFINITY);
-        for (int j = 0; j < a.n_top; j++) {           /* the lists are sorted: past the last taker nothing follows */
+        top.threshold(have ? lp_val((uint32_t)(key[0] >> 32)) : -INFINITY);
+        /* the lists are sorted: past the first entry that nobody takes nothing follows */
+#pragma unroll 1
+        for (int j = 0; j < a.n_top; j++) {
             const bool ok = j < have;
-            const float v = ok ? pv[j] : -INFINITY;
-            const int i = ok ? pi[j] : 0x7fffffff;
-            if (!__builtin_amdgcn_ballot_w64(ok && lp_before(v, i, top.tv, top.ti))) break;
-            top.offer(v, i, ok);
+            if (!__builtin_amdgcn_ballot_w64(ok && key[0] > top.t)) break;
+            top.offer(key[0], ok);
+#pragma unroll
+            for (int u = 0; u + 1 < U; u++) key[u] = key[u + 1];
+            key[U - 1] = pk[min(j + U, a.n_top - 1)];
         }
         if (top.cnt) top.compact();
     }
