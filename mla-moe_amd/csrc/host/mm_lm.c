@@ -93,7 +93,7 @@ int mm_token_logprobs_dev(mm_ctx *c, int T, const float *logits, size_t stride, 
         (st = mm_call_workspace(c, "mm_token_logprobs_dev", ws, ws_bytes, n_s + n_k, (void **)&p)))
         return st;
     mm_logprobs_args a = {logits, stride, targets, logprob, entropy, top_idx, top_logprob,
-                          (float *)p, (uint64_t *)(p + n_s), n, n_top, nseg, seg};
+                          (float *)p, p ? (uint64_t *)(p + n_s) : NULL, n, n_top, nseg, seg};
     const int vec = (uintptr_t)logits % 16 == 0 && (T == 1 || stride % 4 == 0);
     if ((st = mm_launch(c, vec ? K_LOGPROBS : K_LOGPROBS_1, (unsigned)T * (unsigned)nseg, 1, 1, 256, 0, &a)))
         return st;

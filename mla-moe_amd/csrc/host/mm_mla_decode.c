@@ -39,7 +39,7 @@ typedef struct {
  * keys over 64 (or up to 32) rows -- queries, first loads, two tiles until all
  * roles run, its output --, and of the partials written and read back (4 KB per
  * row and chunk at 4 TB/s). */
-static double tiles_us(int t, int nrows) { return (nrows > 32 ? 1.9 : 1.2) * t + 9.0; }
+static double tiles_us(int t, int nrows) { return (nrows > 32 ? 1.7 : 1.1) * t + 9.0; }
 
 static void tiles_chunks(int R, int NH, int rows, int prefix, int own, decode_plan *p) {
     const size_t nrt = ((size_t)R * NH + 63) / 64, ort = (size_t)(R / rows) * ((rows * NH + 63) / 64);
@@ -102,7 +102,7 @@ static int attend(mm_ctx *c, const decode_plan *p, const decode_keys *k, const u
                   float *ml, float *po) {
     const mm_mla_config *g = &c->mla;
     const int NH = g->n_heads, M = n * NH, rows = n < k->rows ? n : k->rows, nseq = n / rows;
-    mm_mla_tiles_args a = {qf, r0 * NH, g->softmax_scale, ml, po, M, NH, p->HG, p->np + p->no,
+    mm_mla_tiles_args a = {qf, r0 * NH, ml, po, M, NH, p->HG, p->np + p->no,
                            k->prefix, k->prefix_len, p->pchunk, p->np, k->cache, k->kv_lens, k->kv_len, k->seq_stride,
                            r0 / k->rows, nseq, rows, p->ochunk, p->no, k->rows, r0 % k->rows, k->sinks, k->window};
     const unsigned np = (unsigned)((M + 63) / 64) * (unsigned)p->np;
@@ -118,7 +118,8 @@ static int decode_run(mm_ctx *c, int layer, const decode_plan *p, const float *q
     uint16_t *qf = (uint16_t *)ws;
     float *ml = (float *)(ws + p->o_ml), *po = (float *)(ws + p->o_po);
     const uint16_t *kv_b = c->mla_kvb[layer];
-    mm_mla_qfrag_args qa = {q, kv_b + (size_t)NH * (QKN + VHD) * MM_MLA_KVL, qf, R, NH, QKN};
+    mm_mla_qfrag_args qa = {q, kv_b + (size_t)NH * (QKN + VHD) * MM_MLA_KVL, qf, R, NH, QKN,
+                            g->softmax_scale * 1.44269504088896341f};
     const unsigned hg8 = (unsigned)(NH + 7) / 8;
     int st;
     if (R < 48)

@@ -498,11 +498,11 @@ typedef struct {
     const uint16_t *wukT;     /* [NH, KVL, QKN] */
     uint16_t *qf;             /* [ceil(R NH / 32)] tiles of MM_MLA_QF_TILE bytes */
     int R, NH, QKN;
+    float scale2;             /* softmax scale / ln 2, taken into the queries */
 } mm_mla_qfrag_args;
 typedef struct {
     const uint16_t *qf;       /* the call's queries (mm_mla_qfrag) */
     int row0;                 /* the launch's first row among them */
-    float scale;
     float *part_ml;           /* [M / NH, HG, pchunks, 2, 16] */
     float *part_o;            /* [M / NH, HG, pchunks, 16, KVL] */
     int M, NH, HG, pchunks;

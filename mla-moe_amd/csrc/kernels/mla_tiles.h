@@ -12,12 +12,18 @@
  *   waves 0, 1   scores of tile t + 2 over latents 0..287 (32 rows each)
  *   waves 2, 3   scores of tile t + 1 over latents 288..575, added to the former;
  *                softmax; the probabilities as bf16 pairs to LDS
- *   waves 4..7   O += P V of tile t, 64 rows x 128 latent columns each; and the
- *                loads of the tiles to come
+ *   waves 4..7   O += P V of tile t, 64 rows x 160 (4, 5) or 96 (6, 7) latent
+ *                columns; and the loads of the tiles to come
  * A score wave keeps its 32 rows' queries over its half of the latents (144
- * registers), an output wave its 64 x 128 of O (128 registers): neither would
+ * registers), an output wave up to 64 x 160 of O (160 registers): neither would
  * fit beside the other, and the softmax of one tile runs beside the products of
- * the others.  One barrier per tile.
+ * the others.  One barrier per tile.  Waves 2 and 3 do the softmax, so the output
+ * waves on their SIMDs have fewer columns (128 each: 31 us where this takes 29, 64
+ * rows of 16 heads over 4,096 keys).
+ *
+ * The matrix cores bound it: 2,176 cycles of products a tile on each of four
+ * SIMDs on average, 64 rows of 16 heads over 32,768 keys 130 us in all, 1.12
+ * PFLOP/s of pair products (a library's product of 8,192^3: 1.21).
  *
  * LDS, per tile of 32 keys: latents 0..287 (576 bytes a row, four tiles of
  * them), 288..511 (448 bytes, three), k_pe (128 bytes, two): a part lives until
@@ -51,6 +57,30 @@ __device__ __forceinline__ void tl_barrier() {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
+}
+
+/* acc += K Qhi^T + K Qlo^T over 18 steps of 16 latents, K operands at LDS
+ * addresses addr(s), three steps' reads ahead of the products (without the scheduling
+ * barriers each read sat right before its products). */
+template <class Addr>
+__device__ __forceinline__ void tl_scores(const i32x4 (&qh)[18], const i32x4 (&ql)[18], f32x16 &acc, Addr addr) {
+    i32x4 k[2][3];
+#pragma unroll
+    for (int i = 0; i < 3; i++) k[0][i] = *(lds_w4)(uintptr_t)addr(i);
+#pragma unroll
+    for (int b = 0; b < 6; b++) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (b < 5) {
+#pragma unroll
+            for (int i = 0; i < 3; i++) k[(b + 1) & 1][i] = *(lds_w4)(uintptr_t)addr(3 * (b + 1) + i);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 3; i++) {
+            acc = mfma32(k[b & 1][i], qh[3 * b + i], acc);
+            acc = mfma32(k[b & 1][i], ql[3 * b + i], acc);
+        }
+    }
 }
 
 /* A block's rows and keys. */
@@ -132,7 +162,7 @@ __device__ __forceinline__ void tl_block(const mm_mla_tiles_args &a) {
 
     if (w >= 4) {
         /* ---- O += P V, and the loads ---- */
-        const int bw = w - 4;
+        const int bw = w - 4, cb = bw < 2 ? 5 * bw : 10 + 3 * (bw - 2);   /* its first column tile of the 16 */
         const rsrc_t rk = raw_rsrc(j.keys, (uint32_t)(WIN ? j.len : j.nk) * KVD * 2);
         /* this wave's nine of a tile's 36 1-KB loads: LDS piece x (16 bytes) of
          * the part is row x / pieces-per-row, slot x % it */
@@ -190,23 +220,18 @@ __device__ __forceinline__ void tl_block(const mm_mla_tiles_args &a) {
         /* transposing reads: lane i of 16-lane group g supplies row 4 (4 s + 2 e
          * + g / 2) + i / 4, 4 columns from 16 (g % 2) + 4 (i % 4) of column tile ct */
         const int i16 = lane & 15, gq = lane >> 4, h = gq >> 1;
-        uint32_t va[4][2][2];                          /* [ct][s][e], without the tile's place */
+        uint32_t v0[2], v1[2];                         /* [e], of latents 0..287 and 288.., column tile 0, s = 0 */
 #pragma unroll
-        for (int ct = 0; ct < 4; ct++)
-#pragma unroll
-            for (int s = 0; s < 2; s++)
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const int col4 = 4 * bw + ct;      /* 32-column tile of the 16 */
-                    const bool r0 = col4 < 9;
-                    const int r = 16 * s + 8 * e + 4 * h + (i16 >> 2);
-                    const int low = (2 * (gq & 1) + ((i16 >> 1) & 1)) ^ (2 * e + h);
-                    va[ct][s][e] = lds0 + (r0 ? 0 : TL_O1) + (uint32_t)(r * (r0 ? 576 : 448) + 64 * (r0 ? col4 : col4 - 9) + 16 * low + 8 * (i16 & 1));
-                }
+        for (int e = 0; e < 2; e++) {
+            const int r = 8 * e + 4 * h + (i16 >> 2);
+            const int low = (2 * (gq & 1) + ((i16 >> 1) & 1)) ^ (2 * e + h);
+            v0[e] = lds0 + (uint32_t)(r * 576 + 16 * low + 8 * (i16 & 1));
+            v1[e] = lds0 + TL_O1 + (uint32_t)(r * 448 + 16 * low + 8 * (i16 & 1));
+        }
         const uint32_t pa = lds0 + TL_OP + (uint32_t)(c32 * 64 + 16 * (hi ^ ((c32 >> 2) & 3)));   /* piece 2 s + hi: s flips bit 1 */
-        auto run = [&](auto rtc) {
-            constexpr int RT = decltype(rtc)::value;   /* row tiles */
-            f32x16 O[RT][4] = {};
+        auto run = [&](auto rtc, auto ctc) {
+            constexpr int RT = decltype(rtc)::value, CT = decltype(ctc)::value;   /* row tiles, column tiles */
+            f32x16 O[RT][CT] = {};
             for (int t = 0; t < nt; t++) {
                 if (t + 3 < nt) issue0(t + 3);
                 if (t + 2 < nt) issue1(t + 2);
@@ -220,31 +245,14 @@ __device__ __forceinline__ void tl_block(const mm_mla_tiles_args &a) {
                      * zeroed */
                     uint32_t bad = (uint32_t)__builtin_amdgcn_readfirstlane(flags[2] | (RT > 1 ? flags[3] : 0));
                     while (bad) {
-                        const int r = __builtin_ctz(bad), p = 16 * bw + lane;
+                        const int r = __builtin_ctz(bad), p = 4 * cb + lane;
                         bad &= bad - 1;
-                        if (lane < 16) {
+                        if (lane < 4 * CT) {
                             const uint32_t o = p < 36 ? d0 + r * 576 + 16 * ((p & ~3) | ((p ^ (r >> 2)) & 3))
                                                       : TL_O1 + d1 + r * 448 + 16 * (((p - 36) & ~3) | ((p ^ (r >> 2)) & 3));
                             *(lds_w4)(uintptr_t)(lds0 + o) = (i32x4){0, 0, 0, 0};
                         }
                         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                    }
-                }
-                i32x4 ph[2][RT], pl[2][RT], v[2][4];
-#pragma unroll
-                for (int s = 0; s < 2; s++) {
-#pragma unroll
-                    for (int rt = 0; rt < RT; rt++) {
-                        const uint32_t p = (pa ^ (uint32_t)(32 * s)) + po + 2048 * rt;
-                        ph[s][rt] = *(lds_w4)(uintptr_t)p;
-                        pl[s][rt] = *(lds_w4)(uintptr_t)(p + 4096);
-                    }
-#pragma unroll
-                    for (int ct = 0; ct < 4; ct++) {
-                        const uint32_t d = 4 * bw + ct < 9 ? d0 : d1;
-                        const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(uintptr_t)(va[ct][s][0] + d));
-                        const s16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(uintptr_t)(va[ct][s][1] + d));
-                        v[s][ct] = __builtin_bit_cast(i32x4, (s16x8){x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]});
                     }
                 }
 #pragma unroll
@@ -254,21 +262,39 @@ __device__ __forceinline__ void tl_block(const mm_mla_tiles_args &a) {
                         for (int g = 0; g < 4; g++) {
                             const f32x4 f = *(lds_f4)(uintptr_t)(lds0 + TL_OF + (uint32_t)((t & 1) * 256 + 4 * (32 * rt + 8 * g + 4 * hi)));
 #pragma unroll
-                            for (int ct = 0; ct < 4; ct++)
+                            for (int ct = 0; ct < CT; ct++)
 #pragma unroll
                                 for (int i = 0; i < 4; i++) O[rt][ct][4 * g + i] *= f[i];
                         }
                     }
                 }
 #pragma unroll
-                for (int s = 0; s < 2; s++)
+                for (int s = 0; s < 2; s++) {
+                    i32x4 ph[RT], pl[RT], v[CT];
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int ct = 0; ct < 4; ct++)
+                    for (int rt = 0; rt < RT; rt++) {
+                        const uint32_t p = (pa ^ (uint32_t)(32 * s)) + po + 2048 * rt;
+                        ph[rt] = *(lds_w4)(uintptr_t)p;
+                        pl[rt] = *(lds_w4)(uintptr_t)(p + 4096);
+                    }
 #pragma unroll
-                        for (int rt = 0; rt < RT; rt++) {
-                            O[rt][ct] = mfma32(ph[s][rt], v[s][ct], O[rt][ct]);
-                            O[rt][ct] = mfma32(pl[s][rt], v[s][ct], O[rt][ct]);
-                        }
+                    for (int ct = 0; ct < CT; ct++) {
+                        const int col = cb + ct;       /* 32-column tile of the 16 */
+                        const uint32_t o = col < 9 ? d0 + 64 * col + 16 * 576 * s : d1 + 64 * (col - 9) + 16 * 448 * s;
+                        const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(uintptr_t)((col < 9 ? v0[0] : v1[0]) + o));
+                        const s16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(uintptr_t)((col < 9 ? v0[1] : v1[1]) + o));
+                        v[ct] = __builtin_bit_cast(i32x4, (s16x8){x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]});
+                    }
+                    /* an accumulator's next product CT RT products later */
+#pragma unroll
+                    for (int lo = 0; lo < 2; lo++)
+#pragma unroll
+                        for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                            for (int rt = 0; rt < RT; rt++) O[rt][ct] = mfma32(lo ? pl[rt] : ph[rt], v[ct], O[rt][ct]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
                 VMCNT_WAIT(0);                         /* the loads of this step, a step's products ago */
                 tl_barrier();
             }
@@ -280,9 +306,9 @@ __device__ __forceinline__ void tl_block(const mm_mla_tiles_args &a) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         if (32 * rt + 8 * g + 4 * hi + i >= j.nrows) continue;
-                        float *o = a.part_o + (size_t)(uint32_t)at[i] * KVL + 128 * bw + c32;
+                        float *o = a.part_o + (size_t)(uint32_t)at[i] * KVL + 32 * cb + c32;
 #pragma unroll
-                        for (int ct = 0; ct < 4; ct++) o[32 * ct] = O[rt][ct][4 * g + i];
+                        for (int ct = 0; ct < CT; ct++) o[32 * ct] = O[rt][ct][4 * g + i];
                     }
                 }
         };
@@ -306,8 +332,14 @@ __device__ __forceinline__ void tl_block(const mm_mla_tiles_args &a) {
         tl_barrier();
         VMCNT_WAIT(0);
         tl_barrier();
-        if (two) run(std::integral_constant<int, 2>());
-        else run(std::integral_constant<int, 1>());
+        using std::integral_constant;
+        if (bw < 2) {
+            if (two) run(integral_constant<int, 2>(), integral_constant<int, 5>());
+            else run(integral_constant<int, 1>(), integral_constant<int, 5>());
+        } else {
+            if (two) run(integral_constant<int, 2>(), integral_constant<int, 3>());
+            else run(integral_constant<int, 1>(), integral_constant<int, 3>());
+        }
         return;
     }
 
@@ -335,17 +367,13 @@ __device__ __forceinline__ void tl_block(const mm_mla_tiles_args &a) {
         const uint32_t e0 = ka + 16 * (hi ^ sw), e1 = ka + 16 * ((2 + hi) ^ sw);   /* steps 0, 2, ..; 1, 3, .. */
         for (int t = 0; t < nt; t++) {
             const uint32_t d = (uint32_t)(t & 3) * TL_R0;
-            f32x16 s1 = {}, s2 = {};
-#pragma unroll
-            for (int s = 0; s < 18; s++) {
-                const i32x4 k = *(lds_w4)(uintptr_t)((s & 1 ? e1 : e0) + d + 64 * (s >> 1));
-                s1 = mfma32(k, qh[s], s1);
-                s2 = mfma32(k, ql[s], s2);
-            }
+            f32x16 s = {};
+            const uint32_t a0 = e0 + d, a1 = e1 + d;
+            tl_scores(qh, ql, s, [&](int i) { return (i & 1 ? a1 : a0) + 64 * (i >> 1); });
 #pragma unroll
             for (int i = 0; i < 4; i++)
                 *(lds_f4)(uintptr_t)(xa + (uint32_t)((t & 1) * 8192 + 1024 * i)) =
-                    (f32x4){s1[4 * i] + s2[4 * i], s1[4 * i + 1] + s2[4 * i + 1], s1[4 * i + 2] + s2[4 * i + 2], s1[4 * i + 3] + s2[4 * i + 3]};
+                    (f32x4){s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]};
             tl_barrier();
         }
         tl_barrier();
@@ -358,7 +386,6 @@ __device__ __forceinline__ void tl_block(const mm_mla_tiles_args &a) {
 #pragma unroll
     for (int s = 0; s < 4; s++) pe[s] = kp + 16 * ((2 * s + hi) ^ ((c32 >> 1) & 7));
     const uint32_t pw = lds0 + TL_OP + (uint32_t)((32 * rh + c32) * 64 + 16 * (hi ^ sw));
-    const float scale2 = a.scale * 1.44269504088896341f;   /* scores in units of ln 2 */
     /* WIN: this lane's position, and those of the block's first and last rows */
     const int pos = WIN ? j.pos0 + (j.first_row + min(32 * rh + c32, j.nrows - 1)) / a.NH : 0;
     const int pos_a = WIN ? j.pos0 + j.first_row / a.NH : 0, pos_b = WIN ? j.pos0 + (j.first_row + j.nrows - 1) / a.NH : 0;
@@ -366,16 +393,15 @@ __device__ __forceinline__ void tl_block(const mm_mla_tiles_args &a) {
     tl_barrier();
     for (int t = 0; t < nt; t++) {
         const uint32_t d = (uint32_t)(t % 3) * TL_R1, dk = (uint32_t)(t & 1) * TL_KP;
-        f32x4 x[4];
+        f32x16 s1;                                     /* scores in units of ln 2 */
 #pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = *(lds_f4)(uintptr_t)(xa + (uint32_t)((t & 1) * 8192 + 1024 * i));
-        f32x16 s1 = {}, s2 = {};
+        for (int i = 0; i < 4; i++) {                  /* the first half's sums */
+            const f32x4 x = *(lds_f4)(uintptr_t)(xa + (uint32_t)((t & 1) * 8192 + 1024 * i));
 #pragma unroll
-        for (int s = 0; s < 18; s++) {
-            const i32x4 k = s < 14 ? *(lds_w4)(uintptr_t)((s & 1 ? e1 : e0) + d + 64 * (s >> 1)) : *(lds_w4)(uintptr_t)(pe[s - 14] + dk);
-            s1 = mfma32(k, qh[s], s1);
-            s2 = mfma32(k, ql[s], s2);
+            for (int q = 0; q < 4; q++) s1[4 * i + q] = x[q];
         }
+        const uint32_t a0 = e0 + d, a1 = e1 + d;
+        tl_scores(qh, ql, s1, [&](int i) { return i < 14 ? (i & 1 ? a1 : a0) + 64 * (i >> 1) : pe[i - 14] + dk; });
         uint32_t bad = 0;
         bool all = true;                               /* uniform: every row sees every key of the tile */
         if (WIN) {
@@ -386,8 +412,6 @@ __device__ __forceinline__ void tl_block(const mm_mla_tiles_args &a) {
             all = 32 * t + 31 < j.nk;
         }
         float mx = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 16; i++) s1[i] = (s1[i] + s2[i] + x[i >> 2][i & 3]) * scale2;
         if (!all) {
             uint32_t own = 0;                          /* this lane's keys that are not finite */
 #pragma unroll
@@ -453,17 +477,18 @@ __device__ __forceinline__ void tl_block(const mm_mla_tiles_args &a) {
     tl_barrier();
 }
 
-/* Absorbed queries and q_pe as the score waves read them: bf16 pairs in 32-row
+/* Absorbed queries and q_pe, times softmax scale / ln 2 (scores come out in units
+ * of ln 2), as the score waves read them: bf16 pairs in 32-row
  * tiles [hi, lo][72 pieces of 8 latents][32 rows][16 bytes], so that a wave's load
  * is 1 KB.  (From row-major planes each load met 32 lines, 2 us per block.)
  *
  * W_UK comes first, as two 16-row tiles whose rows are latents 8 g + i and 8 g +
  * 4 + i (row 4 g + i), so that a lane ends with the 8 latents of a piece. */
-__device__ __forceinline__ void qf_split(const f32x4 &x0, const f32x4 &x1, i32x4 &ph, i32x4 &pl) {
+__device__ __forceinline__ void qf_split(const f32x4 &x0, const f32x4 &x1, float f, i32x4 &ph, i32x4 &pl) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         uint32_t vh, vl;
-        split_pk(i < 2 ? x0[2 * i] : x1[2 * i - 4], i < 2 ? x0[2 * i + 1] : x1[2 * i - 3], &vh, &vl);
+        split_pk((i < 2 ? x0[2 * i] : x1[2 * i - 4]) * f, (i < 2 ? x0[2 * i + 1] : x1[2 * i - 3]) * f, &vh, &vl);
         ph[i] = (int)vh;
         pl[i] = (int)vl;
     }
@@ -507,7 +532,7 @@ __device__ __forceinline__ void qf_wave(const mm_mla_qfrag_args &a, int h, const
 #pragma unroll
             for (int x = 0; x < NX; x++) {
                 i32x4 xh, xl;
-                qf_split(xv[u][x][0], xv[u][x][1], xh, xl);
+                qf_split(xv[u][x][0], xv[u][x][1], 1.0f, xh, xl);
 #pragma unroll
                 for (int s = 0; s < S; s++)
 #pragma unroll
@@ -521,7 +546,7 @@ __device__ __forceinline__ void qf_wave(const mm_mla_qfrag_args &a, int h, const
 #pragma unroll
     for (int s = 0; s < S; s++)
 #pragma unroll
-        for (int x = 0; x < NX; x++) qf_split(y[s][x][0], y[s][x][1], ph[s][x], pl[s][x]);
+        for (int x = 0; x < NX; x++) qf_split(y[s][x][0], y[s][x][1], a.scale2, ph[s][x], pl[s][x]);
 }
 
 /* Few positions: grid (KVL / 64 slabs and one for q_pe, NH, ceil(R / 32)), wave w
@@ -535,7 +560,7 @@ extern "C" __global__ __launch_bounds__(256) void mm_mla_qfrag(mm_mla_qfrag_args
         b = blockIdx.z * 32 + (tid >> 3);
         piece = KVL / 8 + (tid & 7);
         const float *q = a.q + ((size_t)min(b, a.R - 1) * a.NH + h) * (a.QKN + MM_MLA_QKR) + a.QKN + 8 * (tid & 7);
-        qf_split(*(const f32x4 *)q, *(const f32x4 *)(q + 4), ph[0][0], pl[0][0]);
+        qf_split(*(const f32x4 *)q, *(const f32x4 *)(q + 4), a.scale2, ph[0][0], pl[0][0]);
     } else {
         const int e0 = 64 * slab + 32 * (w & 1);
         b = blockIdx.z * 32 + 16 * (w >> 1) + (lane & 15);
@@ -568,7 +593,7 @@ __device__ __forceinline__ void qf_block(const mm_mla_qfrag_args &a) {
             if (b >= a.R || h0 + sh >= a.NH) continue;
             const float *q = a.q + ((size_t)b * a.NH + h0 + sh) * (a.QKN + MM_MLA_QKR) + a.QKN + 8 * piece;
             i32x4 ph, pl;
-            qf_split(*(const f32x4 *)q, *(const f32x4 *)(q + 4), ph, pl);
+            qf_split(*(const f32x4 *)q, *(const f32x4 *)(q + 4), a.scale2, ph, pl);
             uint8_t *p = qf_place(a, b, h0 + sh, KVL / 8 + piece);
             *(i32x4 *)p = ph;
             *(i32x4 *)(p + MM_MLA_QF_TILE / 2) = pl;
@@ -667,7 +692,7 @@ __device__ __forceinline__ void merge_uv(const mm_mla_merge_uv_args &a) {
             const float wc = cb + lane < a.nchunks && mc != -INFINITY ? __expf(mc - mx) : 0.0f;
             l += lc * wc;
             const int n = min(MM_WAVE, a.nchunks - cb);
-            constexpr int U = 8;                       /* chunks whose loads are in flight */
+            constexpr int U = 4;                       /* chunks whose loads are in flight */
             for (int c0 = cg; c0 < n; c0 += U * G) {
                 f32x4 v[U][2];
 #pragma unroll
@@ -679,8 +704,7 @@ __device__ __forceinline__ void merge_uv(const mm_mla_merge_uv_args &a) {
 #pragma unroll
                 for (int u = 0; u < U; u++) {
                     const int c = c0 + u * G;
-                    if (c >= n) break;                 /* uniform */
-                    const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wc), c));
+                    const float f = c < n ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wc), c & 63)) : 0.0f;
                     s0 += v[u][0] * f;
                     s1 += v[u][1] * f;
                 }
