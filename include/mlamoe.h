@@ -342,7 +342,7 @@ MM_API int mm_lm_head_dev(mm_ctx *ctx, int B, const float *x, const uint16_t *no
  *   top_idx, top_logprob    [T, n_top] the n_top largest logits' tokens and log
  *                           probabilities, descending, of equal ones (-0 and 0
  *                           too) the lowest token first
- * n_top <= 32 and <= n; n <= 2^30.  A row's -inf logits are tokens of
+ * n_top <= 32 and <= n; n <= 2^30, T <= 2^23.  A row's -inf logits are tokens of
  * probability 0, listed after every other.  NaN logits are never listed: with
  * fewer than n_top numbers in a row the rest is -1 and NaN.  A row that holds a
  * NaN or +inf, or nothing above -inf, has no distribution: its logprob, entropy

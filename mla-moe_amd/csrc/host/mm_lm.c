@@ -56,8 +56,8 @@ static int logprobs_seg(int T, int n, int *nseg) {
 static int logprobs_check(int T, int n, int n_top) {
     if (T < 0 || n <= 0 || n_top < 0 || n_top > n)
         return mm_fail(MM_ERR_INVALID, "mm_token_logprobs: bad shape");
-    if (n_top > MM_LP_TOP_MAX || n > 1 << 30)
-        return mm_fail(MM_ERR_UNSUPPORTED, "mm_token_logprobs: n_top <= %d, n <= 2^30", MM_LP_TOP_MAX);
+    if (n_top > MM_LP_TOP_MAX || n > 1 << 30 || T > 1 << 23)
+        return mm_fail(MM_ERR_UNSUPPORTED, "mm_token_logprobs: n_top <= %d, n <= 2^30, T <= 2^23", MM_LP_TOP_MAX);
     return MM_OK;
 }
 
@@ -85,8 +85,6 @@ int mm_token_logprobs_dev(mm_ctx *c, int T, const float *logits, size_t stride, 
     if (T == 0 || (!logprob && !entropy && n_top == 0)) return MM_OK;
     if ((st = mm_set_device(c))) return st;
     const int seg = logprobs_seg(T, n, &nseg);
-    if ((size_t)T * nseg > 0x7fffffffu)
-        return mm_fail(MM_ERR_UNSUPPORTED, "mm_token_logprobs_dev: %d rows of %d", T, n);
     char *p = NULL;
     const size_t n_s = al256((size_t)T * nseg * 16), n_k = (size_t)T * nseg * n_top * 8;
     if (nseg > 1 &&

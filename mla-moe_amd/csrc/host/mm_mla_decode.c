@@ -149,7 +149,7 @@ static int decode_run(mm_ctx *c, int layer, const decode_plan *p, const float *q
         const int split = R >= 256 ? 1 : (ncol + nw - 1) / nw;
         int ppb = R >= 256 ? 16 : 4, wpp = 1;
         if (R > 16 && R < 256 && (size_t)NH * ((R + 3) / 4) * split > 256) ppb = 8;
-        while (2 * wpp * R <= nw) wpp *= 2;
+        while (2 * wpp * R <= nw) wpp *= 2;          /* by the call's rows: the same bits in groups */
         const int rt = (n + ppb - 1) / ppb;
         mm_mla_merge_uv_args ma = {ml, po, kv_b, ctx_out + h0 * VHD, n, NH, p->HG, QKN, VHD, p->np + p->no,
                                    ppb, split, wpp};

@@ -676,9 +676,11 @@ __device__ __forceinline__ void merge_uv(const mm_mla_merge_uv_args &a) {
     }
 #pragma unroll
     for (int ri = 0; ri < 16 / NW; ri++) {
+        /* G > 1: one round, in which waves past the rows (a call's last group of
+         * rows) repeat the last one, since all meet at the barrier */
         const int r = w / G + ri * (NW / G);
-        if (r >= nrows) break;
-        const size_t pb = ((size_t)(b0 + r) * a.HG + (h >> 4)) * a.nchunks;
+        if (G > 1 ? ri > 0 : r >= nrows) break;
+        const size_t pb = ((size_t)(b0 + min(r, nrows - 1)) * a.HG + (h >> 4)) * a.nchunks;
         const float *ml = a.part_ml + pb * 32 + (h & 15);
         const float *po = a.part_o + (pb * 16 + (h & 15)) * KVL + 4 * lane;
         float mx = mcs[ri];                            /* lanes past the chunks hold the last one's */

@@ -274,3 +274,9 @@ def test_refusals_without_a_gpu():
         assert b.value == 0
     assert mlamoe.token_logprobs_workspace(4000, 102400, 20) == 0     # a row a block: none needed
     assert mlamoe.token_logprobs_workspace(1, 102400, 20) > 0
+
+
+def test_more_rows_than_a_grid_holds_are_refused():
+    b = C.c_size_t(7)
+    assert mlamoe.lib().mm_token_logprobs_workspace((1 << 23) + 1, 10, 1, C.byref(b)) == -2 and b.value == 0
+    assert mlamoe.token_logprobs_workspace(1 << 23, 10, 1) == 0

@@ -260,6 +260,43 @@ def test_window_rows_in_groups(monkeypatch):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("NH,B", [(64, 2), (128, 1), (32, 2), (64, 3)])
+def test_few_rows_in_groups(monkeypatch, NH, B):
+    """Few rows of many heads, whose merge shares a row's chunks between waves:
+    one row per group, the same bits."""
+    a = prefix_case(NH, B, 1500, 40, [40 - b for b in range(B)], QKN=64, VHD=32, seed=43)
+    w = window_case(NH, 1, B, 700, 3, 500, QKN=64, VHD=32, seed=44)
+    monkeypatch.setenv("MLAMOE_MLA_PART_MAX", "1")
+    assert np.array_equal(a, prefix_case(NH, B, 1500, 40, [40 - b for b in range(B)], QKN=64, VHD=32, seed=43))
+    assert np.array_equal(w, window_case(NH, 1, B, 700, 3, 500, QKN=64, VHD=32, seed=44))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [0x7FC0, 0x7F80, 0xFF80])
+def test_window_keys_that_are_not_finite(bad):
+    """A drafted position whose cache row is not finite: the rows before it,
+    which do not see it, are what they are without it; the rows that see it have
+    no finite value.  So does a key that has left some rows' windows."""
+    NH, B, rows, L, sinks, window = 16, 2, 9, 300, 2, 70
+    rng = np.random.default_rng(45)
+    q = synth.normal_f32(rng, (B, rows, NH, 192), 2.0)
+    cache = synth.normal_bf16(rng, (B, L, KVL + QKR), 1.0)
+    clean = cache.copy()
+    new, old = L - rows + 5, L - rows + 3 - window + 1           # rows 5.. see `new`, rows ..3 `old`
+    cache[0, new] = np.uint16(bad)
+    cache[1, old] = np.uint16(bad)
+    ctx, _ = loaded(NH)
+    with ctx:
+        got, want = ctx.mla_window_decode(0, q, cache, sinks, window), ctx.mla_window_decode(0, q, clean, sinks, window)
+    for r in range(rows):
+        for b, sees in ((0, r >= 5), (1, r <= 3)):
+            if sees:
+                assert not np.isfinite(got[b, r]).any(), (b, r)
+            else:
+                assert np.array_equal(got[b, r], want[b, r]), (b, r)
+
+
+@pytest.mark.gpu
 def test_far_caches():
     """Own rows past 2^32 bytes of the caches."""
     NH, B, stride, P = 16, 260, 16384, 100
@@ -324,6 +361,41 @@ def test_captured():
             for a, b in zip(out[:2], out[2:]):
                 assert np.array_equal(a.download(), b.download()), rep
         g.close()
+
+
+@pytest.mark.gpu
+def test_callers_stream_and_rows_behind():
+    """On a stream of the caller's: the same bits as on the context's, and
+    nothing behind the last row or the workspace is written."""
+    NH, B, P, L = 16, 5, 260, 33
+    rng = np.random.default_rng(92)
+    q, prefix = synth.normal_f32(rng, (B, NH, 192)), synth.normal_bf16(rng, (P, 576), 1.0)
+    cache, lens = synth.normal_bf16(rng, (B, L, 576), 1.0), np.array([33, 0, 7, 32, 1], np.int32)
+    ctx, _ = loaded(NH)
+    hip = C.CDLL("libamdhip64.so")
+    stream = C.c_void_p()
+    hip.hipStreamCreateWithFlags.argtypes = [C.POINTER(C.c_void_p), C.c_uint]
+    hip.hipStreamDestroy.argtypes = [C.c_void_p]
+    with ctx:
+        a, w = ctx.mla_prefix_decode(0, q, prefix, cache, lens), ctx.mla_window_decode(0, q[:, None], cache, 1, 9, lens)
+        dq, dp, dc, dl = (ctx.to_device(v) for v in (q, prefix, cache, lens))
+        need = max(ctx.mla_prefix_decode_workspace(B, P, L), ctx.mla_window_decode_workspace(B, 1, L, 1, 9))
+        out, ws = ctx.to_device(np.full((B + 2, NH * 128), 7.0, np.float32)), ctx.to_device(np.full(need + 4096, 7, np.uint8))
+        size = ws.nbytes
+        ctx.sync()
+        assert hip.hipStreamCreateWithFlags(C.byref(stream), 1) == 0
+        ctx.set_stream(stream)
+        for want, call in ((a, lambda: ctx.mla_prefix_decode_dev(0, B, dq, dp, P, dc, L, L, out, dl, ws)),
+                           (w[:, 0], lambda: ctx.mla_window_decode_dev(0, B, 1, dq, dc, L, L, 1, 9, out, dl, ws))):
+            ws.nbytes = need
+            call()
+            ws.nbytes = size
+            got = out.download()
+            assert np.array_equal(got[:B], want) and np.all(got[B:] == 7.0)
+            assert np.all(ws.download()[need:] == 7)
+        ctx.set_stream(None)
+        ctx.sync()
+    assert hip.hipStreamDestroy(stream) == 0
 
 
 @pytest.mark.gpu
