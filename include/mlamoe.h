@@ -402,7 +402,8 @@ MM_API int mm_mla_absorbed_decode_dev(mm_ctx *ctx, int layer, int B, const float
  *   q        [B, NH, QKN + QKR] fp32, q_nope | q_pe (RoPE applied, at the
  *            positions after the prefix; so is the own rows' k_pe)
  *   prefix   [prefix_len, KVL + QKR] bf16, or NULL with prefix_len 0
- *   cache    [B, seq_stride, KVL + QKR] bf16, or NULL with kv_len 0
+ *   cache    [B, seq_stride, KVL + QKR] bf16 (appended to by
+ *            mm_mla_front_prefix_dev), or NULL with kv_len 0
  *   kv_lens  [B] own rows of each sequence (taken as within [0, kv_len]), or
  *            NULL: kv_len
  *   ctx_out  [B, NH * VHD] fp32; zeros for a sequence without any key
@@ -515,6 +516,15 @@ typedef struct {
 MM_API int mm_mla_front_dev(mm_ctx *ctx, int B, const float *x, const mm_mla_front_weights *w,
                             const int32_t *pos, float *q, uint16_t *cache, int seq_stride,
                             float *kv_rows);
+
+/* mm_mla_front_dev for sequences behind a shared prefix of prefix_len rows
+ * (mm_mla_prefix_decode_dev): pos[b] counts from the prefix's start and the row
+ * goes to cache[b, pos[b] - prefix_len], the sequence's own; one outside
+ * [prefix_len, prefix_len + seq_stride) writes none.  prefix_len >= 0. */
+MM_API int mm_mla_front_prefix_dev(mm_ctx *ctx, int B, const float *x,
+                                   const mm_mla_front_weights *w, const int32_t *pos,
+                                   int prefix_len, float *q, uint16_t *cache, int seq_stride,
+                                   float *kv_rows);
 
 /* ---- batched decode engine ------------------------------------------------- */
 

@@ -451,7 +451,7 @@ static int run_planned(mm_engine *e, int R, int n_want, int32_t *next, float *lo
         if ((st = mm_mla_front_rows(c, R, e->x, &L->front, d_pos, d_slot, e->q, e->cache[l], e->lcap[l],
                                     NULL, pre ? e->xn : NULL, pre && hl_rows(e, R) ? e->xn_hl : NULL,
                                     fuse ? e->fcomp : NULL,
-                                    fuse ? &ra : NULL)))
+                                    fuse ? &ra : NULL, 0)))
             return st;
         /* expanded rows first, then the others' ranges; all of them as one
          * absorbed range when the GPU has no room for the expanded keys */

@@ -271,11 +271,12 @@ int mm_gemv_launch(mm_ctx *ctx, const mm_gemv_args *a);
  * made; its arguments go to *defer for mm_mla_decode_rows to run with the
  * absorbed queries in one launch, and kv_a's output goes to comp_buf
  * ([B, KVL + QKR] fp32, the caller's) instead of the workspace, which later
- * calls reuse before that launch runs. */
+ * calls reuse before that launch runs.  row0: the position of the caches' first
+ * row. */
 int mm_mla_front_rows(mm_ctx *ctx, int B, const float *x, const mm_mla_front_weights *w,
                       const int32_t *pos, const int32_t *slots, float *q, uint16_t *cache,
                       int seq_stride, float *kv_rows, const float *xn_pre,
-                      const uint16_t *xn_pre_hl, float *comp_buf, mm_mla_rope_args *defer);
+                      const uint16_t *xn_pre_hl, float *comp_buf, mm_mla_rope_args *defer, int row0);
 /* rope (or NULL): the deferred RoPE of mm_mla_front_rows, run with qprep;
  * ctx_hl (or NULL): ctx_out also as bf16 hi/lo planes [2, B, NH * VHD].
  * rows4: slots given and rows 4 j .. 4 j + 3 of every group share a cache

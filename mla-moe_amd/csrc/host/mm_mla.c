@@ -309,13 +309,21 @@ int mm_mla_front_dev(mm_ctx *c, int B, const float *x, const mm_mla_front_weight
                      const int32_t *pos, float *q, uint16_t *cache, int seq_stride,
                      float *kv_rows) {
     return mm_mla_front_rows(c, B, x, w, pos, NULL, q, cache, seq_stride, kv_rows, NULL, NULL, NULL,
-                             NULL);
+                             NULL, 0);
+}
+
+int mm_mla_front_prefix_dev(mm_ctx *c, int B, const float *x, const mm_mla_front_weights *w,
+                            const int32_t *pos, int prefix_len, float *q, uint16_t *cache,
+                            int seq_stride, float *kv_rows) {
+    if (prefix_len < 0) return mm_fail(MM_ERR_INVALID, "mm_mla_front_prefix_dev: prefix_len < 0");
+    return mm_mla_front_rows(c, B, x, w, pos, NULL, q, cache, seq_stride, kv_rows, NULL, NULL, NULL,
+                             NULL, prefix_len);
 }
 
 int mm_mla_front_rows(mm_ctx *c, int B, const float *x, const mm_mla_front_weights *w,
                       const int32_t *pos, const int32_t *slots, float *q, uint16_t *cache,
                       int seq_stride, float *kv_rows, const float *xn_pre,
-                      const uint16_t *xn_pre_hl, float *comp_buf, mm_mla_rope_args *defer) {
+                      const uint16_t *xn_pre_hl, float *comp_buf, mm_mla_rope_args *defer, int row0) {
     if (!c) return mm_fail(MM_ERR_INVALID, "mm_mla_front_dev: NULL context");
     if (!c->front_ready) return mm_fail(MM_ERR_STATE, "mm_mla_front_dev: call mm_mla_front_init first");
     if (B < 0) return mm_fail(MM_ERR_INVALID, "mm_mla_front_dev: B < 0");
@@ -405,7 +413,7 @@ int mm_mla_front_rows(mm_ctx *c, int B, const float *x, const mm_mla_front_weigh
     }
     mm_mla_rope_args r = {q, comp, w->kv_a_norm, c->front_inv, pos, cache, kv_rows, B, NH,
                           g->qk_nope_head_dim, g->qk_rope_head_dim, g->kv_lora_rank, seq_stride,
-                          f->rope_interleaved, f->mla_norm_eps, slots};
+                          f->rope_interleaved, f->mla_norm_eps, slots, row0};
     if (defer) {
         *defer = r;
         return MM_OK;

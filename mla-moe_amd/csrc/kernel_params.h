@@ -799,6 +799,7 @@ typedef struct {
     int B, nh, qkn, qkr, kvl, seq_stride, interleaved;
     float eps;               /* kv_a_layernorm eps */
     const int32_t *slots;    /* [B] cache sequence of token b, or 0: sequence b */
+    int row0;                /* >= 0: position of the caches' first row */
 } mm_mla_rope_args;
 
 /* RoPE / kv norm / cache append (one block per token) and the absorbed

@@ -1044,10 +1044,10 @@ extern "C" __global__ __launch_bounds__(256) void mm_mla_uv_w(mm_mla_combine_arg
  *   q_pe of every head   rope_apply(q_h + QKN, p)                (run.c:420-421)
  *   c_kv                 rmsnorm(comp[0:KVL], kv_a_layernorm, eps) (run.c:426)
  *   k_pe                 rope_apply(comp[KVL:KVL+QKR], p)         (run.c:427-428)
- * The row c_kv | k_pe goes to the bf16 cache at (b, p), rounded to nearest
+ * The row c_kv | k_pe goes to the bf16 cache at (b, p - row0), rounded to nearest
  * even (the reference keeps an fp32 cache, include/model.h:117), and, when
- * kv_out is given, to kv_out in fp32.  A position outside [0, seq_stride)
- * writes no cache row.  cos / sin of the angle p * inv_freq[j] are evaluated
+ * kv_out is given, to kv_out in fp32.  A position outside [row0, row0 +
+ * seq_stride) writes no cache row.  cos / sin of the angle p * inv_freq[j] are evaluated
  * in fp64 and rounded once, so they are the correctly rounded fp32 values
  * except for angles within ~2^-29 relative of a rounding boundary; the
  * rotations are unfused multiply / add, in the reference's order. */
@@ -1120,8 +1120,8 @@ __device__ __forceinline__ void rope_token(const mm_mla_rope_args &a, int b) {
     }
 
     /* the cache row */
-    const bool wr = p >= 0 && p < a.seq_stride;
-    uint16_t *dst = a.cache + ((size_t)seq * a.seq_stride + (wr ? p : 0)) * kvd;
+    const bool wr = p >= a.row0 && p - a.row0 < a.seq_stride;
+    uint16_t *dst = a.cache + ((size_t)seq * a.seq_stride + (wr ? p - a.row0 : 0)) * kvd;
     float *ko = a.kv_out ? a.kv_out + (size_t)b * kvd : nullptr;
     {
         const int i = 2 * tid;

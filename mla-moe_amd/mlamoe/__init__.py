@@ -181,6 +181,8 @@ def lib():
         L.mm_mla_front_init.argtypes = [_vp, C.POINTER(MlaFrontConfig)]
         L.mm_mla_front_dev.argtypes = [_vp, C.c_int, _vp, C.POINTER(MlaFrontWeights), _vp, _vp,
                                        _vp, C.c_int, _vp]
+        L.mm_mla_front_prefix_dev.argtypes = [_vp, C.c_int, _vp, C.POINTER(MlaFrontWeights), _vp, C.c_int,
+                                              _vp, _vp, C.c_int, _vp]
         _lib = L
     return _lib
 
@@ -723,6 +725,12 @@ class Context:
         _check(lib().mm_mla_front_dev(self.h, B, x.ptr, C.byref(wstruct), pos.ptr, q.ptr,
                                       cache.ptr, seq_stride,
                                       kv_rows.ptr if kv_rows is not None else None))
+
+    def mla_front_prefix_dev(self, B, x, wstruct, pos, prefix_len, q, cache, seq_stride, kv_rows=None):
+        """mm_mla_front_prefix_dev over device buffers."""
+        _check(lib().mm_mla_front_prefix_dev(self.h, B, x.ptr, C.byref(wstruct), pos.ptr, prefix_len, q.ptr,
+                                             cache.ptr, seq_stride,
+                                             kv_rows.ptr if kv_rows is not None else None))
 
     def mla_front(self, x, w, pos, cache):
         """Host arrays: x [B, H] fp32, w a dict of bf16 weights, pos [B],
