@@ -104,7 +104,6 @@ static const struct {
     [K_ROUTE_WIDE] = {"mm_route_wide", MOD_MOE_I8},
     [K_MLA_QFRAG] = {"mm_mla_qfrag", MOD_MLA},
     [K_MLA_QFRAG_8] = {"mm_mla_qfrag_8", MOD_MLA},
-    [K_MLA_QFRAG_W] = {"mm_mla_qfrag_w", MOD_MLA},
     [K_MLA_ATTN_TILES] = {"mm_mla_attn_tiles", MOD_MLA},
     [K_MLA_ATTN_TILES_W] = {"mm_mla_attn_tiles_w", MOD_MLA},
     [K_MLA_MERGE_UV4] = {"mm_mla_merge_uv_4", MOD_MLA},

@@ -81,7 +81,6 @@ typedef enum {
     K_ROUTE_WIDE,
     K_MLA_QFRAG,
     K_MLA_QFRAG_8,
-    K_MLA_QFRAG_W,
     K_MLA_ATTN_TILES,
     K_MLA_ATTN_TILES_W,
     K_MLA_MERGE_UV4,

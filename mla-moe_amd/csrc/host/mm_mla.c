@@ -49,16 +49,18 @@ int mm_mla_load_layer(mm_ctx *c, int layer, const uint16_t *kv_b, unsigned flags
     int st = mm_set_device(c);
     if (st) return st;
     const mm_mla_config *g = &c->mla;
-    /* one pool per layer: kv_b as given, then W_UK^T per head [NH][KVL][QKN] */
+    /* one pool per layer: kv_b as given, then W_UK^T per head [NH][KVL][QKN], then
+     * W_UV in the merge's fragments */
     const size_t n = (size_t)g->n_heads * (g->qk_nope_head_dim + g->v_head_dim) * g->kv_lora_rank;
     const size_t nt = (size_t)g->n_heads * g->kv_lora_rank * g->qk_nope_head_dim;
-    MM_HIP(hipMalloc((void **)&c->mla_kvb[layer], (n + nt) * 2));
+    const size_t nf = (size_t)g->n_heads * ((g->v_head_dim + 15) / 16) * MM_MLA_UVF_TILE;
+    MM_HIP(hipMalloc((void **)&c->mla_kvb[layer], (n + nt + nf) * 2));
     MM_HIP(hipMemcpyAsync(c->mla_kvb[layer], kv_b, n * 2,
                           (flags & MM_LOAD_DEVICE_PTRS) ? hipMemcpyDeviceToDevice
                                                         : hipMemcpyHostToDevice,
                           c->stream));
-    mm_mla_wprep_args wa = {c->mla_kvb[layer], c->mla_kvb[layer] + n, g->n_heads,
-                            g->qk_nope_head_dim, g->v_head_dim};
+    mm_mla_wprep_args wa = {c->mla_kvb[layer], c->mla_kvb[layer] + n, c->mla_kvb[layer] + n + nt,
+                            g->n_heads, g->qk_nope_head_dim, g->v_head_dim};
     if ((st = mm_launch(c, K_MLA_WPREP, 1024, 1, 1, 256, 0, &wa))) return st;
     MM_HIP(hipStreamSynchronize(c->stream));
     return MM_OK;

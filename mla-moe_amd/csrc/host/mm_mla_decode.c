@@ -117,18 +117,15 @@ static int decode_run(mm_ctx *c, int layer, const decode_plan *p, const float *q
     const int NH = g->n_heads, QKN = g->qk_nope_head_dim, VHD = g->v_head_dim, R = p->R;
     uint16_t *qf = (uint16_t *)ws;
     float *ml = (float *)(ws + p->o_ml), *po = (float *)(ws + p->o_po);
-    const uint16_t *kv_b = c->mla_kvb[layer];
-    mm_mla_qfrag_args qa = {q, kv_b + (size_t)NH * (QKN + VHD) * MM_MLA_KVL, qf, R, NH, QKN,
+    const uint16_t *wukT = c->mla_kvb[layer] + (size_t)NH * (QKN + VHD) * MM_MLA_KVL;
+    const uint16_t *wuvf = wukT + (size_t)NH * MM_MLA_KVL * QKN;
+    mm_mla_qfrag_args qa = {q, wukT, qf, R, NH, QKN,
                             g->softmax_scale * 1.44269504088896341f};
-    const unsigned hg8 = (unsigned)(NH + 7) / 8;
     int st;
     if (R < 48)
         st = mm_launch(c, K_MLA_QFRAG, MM_MLA_KVL / 64 + 1, (unsigned)NH, (unsigned)(R + 31) / 32, 256, 0, &qa);
-    else if (R < 256)
-        st = mm_launch(c, K_MLA_QFRAG_8, MM_MLA_KVL / 32 + 1, hg8, (unsigned)(R + 15) / 16, 512, 0, &qa);
     else
-        st = mm_launch(c, K_MLA_QFRAG_W, MM_MLA_KVL / (32 * MM_MLA_QF_S) + 1, hg8,
-                       (unsigned)(R + 16 * MM_MLA_QF_NX - 1) / (16 * MM_MLA_QF_NX), 512, 0, &qa);
+        st = mm_launch(c, K_MLA_QFRAG_8, MM_MLA_KVL / 32 + 1, (unsigned)(NH + 7) / 8, (unsigned)(R + 15) / 16, 512, 0, &qa);
     if (st) return st;
     for (int r0 = 0, n; r0 < R; r0 += n) {
         n = R - r0 < p->G ? R - r0 : p->G;
@@ -151,7 +148,7 @@ static int decode_run(mm_ctx *c, int layer, const decode_plan *p, const float *q
         if (R > 16 && R < 256 && (size_t)NH * ((R + 3) / 4) * split > 256) ppb = 8;
         while (2 * wpp * R <= nw) wpp *= 2;          /* by the call's rows: the same bits in groups */
         const int rt = (n + ppb - 1) / ppb;
-        mm_mla_merge_uv_args ma = {ml, po, kv_b, ctx_out + h0 * VHD, n, NH, p->HG, QKN, VHD, p->np + p->no,
+        mm_mla_merge_uv_args ma = {ml, po, wuvf, ctx_out + h0 * VHD, n, NH, p->HG, VHD, p->np + p->no,
                                    ppb, split, wpp};
         const unsigned blocks = (unsigned)NH * (unsigned)rt * (unsigned)split;
         if ((st = mm_launch(c, nw == 4 ? K_MLA_MERGE_UV4 : K_MLA_MERGE_UV8, blocks, 1, 1, 64 * nw, 0, &ma))) return st;

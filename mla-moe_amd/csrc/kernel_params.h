@@ -447,10 +447,13 @@ typedef struct {
     int B, NH, QKN;
 } mm_mla_qprep_args;
 
-/* Load-time preparation of W_UK^T from the head-interleaved kv_b. */
+/* Load-time preparation of W_UK^T and of W_UV in fragments from the
+ * head-interleaved kv_b. */
+#define MM_MLA_UVF_TILE (16 * 512)   /* elements of 16 columns: [KVL / 32][64 lanes][8] */
 typedef struct {
     const uint16_t *kv_b;
     uint16_t *wukT;
+    uint16_t *wuvf;           /* [NH, ceil(VHD / 16)] tiles */
     int NH, QKN, VHD;
 } mm_mla_wprep_args;
 
@@ -488,10 +491,6 @@ typedef struct {
  * where nchunks is 0), then as many for the N = nseq ceil(rows NH / 64)
  * ochunks of the sequences' own keys. */
 #define MM_MLA_TL_LDS 158720      /* dynamic LDS of a block */
-#ifndef MM_MLA_QF_NX
-#define MM_MLA_QF_NX 2            /* mm_mla_qfrag_w: 16-position and 32-latent tiles per wave */
-#define MM_MLA_QF_S 4
-#endif
 #define MM_MLA_QF_TILE (2 * 72 * 512)   /* bytes of 32 rows' queries: hi and lo, 72 pieces of 8 latents */
 typedef struct {
     const float *q;           /* [R, NH, QKN + QKR] */
@@ -521,9 +520,9 @@ typedef struct {
 /* Their merge and W_UV product (mm_mla_merge_uv_4, _8: waves per block). */
 typedef struct {
     const float *part_ml, *part_o;   /* [R, HG, nchunks, ..] */
-    const uint16_t *kv_b;
+    const uint16_t *wuvf;     /* mm_mla_wprep_args */
     float *ctx;               /* [R, NH * VHD] */
-    int R, NH, HG, QKN, VHD, nchunks;
+    int R, NH, HG, VHD, nchunks;
     int ppb;                  /* positions per block, at most 16 */
     int split;                /* blocks over a head's columns, at most ceil(VHD / 16) */
     int wpp;                  /* waves that share a position: a power of two, wpp R <= waves or 1 */

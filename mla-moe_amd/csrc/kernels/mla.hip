@@ -229,13 +229,24 @@ extern "C" __global__ __launch_bounds__(256) void mm_mla_qprep_w(mm_mla_qprep_ar
     }
 }
 
-/* Load-time: W_UK_h transposed, wukT[h][r][d] = kv_b[h (QKN + VHD) + d][r]. */
+/* Load-time: W_UK_h transposed, wukT[h][r][d] = kv_b[h (QKN + VHD) + d][r]; W_UV_h in
+ * 16-column tiles as a wave's fragments, element i of lane l in step s of tile c is
+ * latent 32 s + 8 (l / 16) + i of column 16 c + l % 16 (past the last: that again). */
 extern "C" __global__ __launch_bounds__(256) void mm_mla_wprep(mm_mla_wprep_args a) {
     const size_t n = (size_t)a.NH * KVL * a.QKN;
     for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n;
          i += (size_t)gridDim.x * blockDim.x) {
         const size_t d = i % a.QKN, r = (i / a.QKN) % KVL, h = i / ((size_t)a.QKN * KVL);
         a.wukT[i] = a.kv_b[(h * (a.QKN + a.VHD) + d) * KVL + r];
+    }
+    const int ncol = (a.VHD + 15) / 16;
+    const size_t nf = (size_t)a.NH * ncol * MM_MLA_UVF_TILE;
+    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < nf;
+         i += (size_t)gridDim.x * blockDim.x) {
+        const int e = (int)(i % MM_MLA_UVF_TILE), l = e >> 3 & 63, r = 32 * (e >> 9) + 8 * (l >> 4) + (e & 7);
+        const size_t c = i / MM_MLA_UVF_TILE, h = c / ncol;
+        const size_t v = min((int)(c % ncol) * 16 + (l & 15), a.VHD - 1);
+        a.wuvf[i] = a.kv_b[(h * (a.QKN + a.VHD) + a.QKN + v) * KVL + r];
     }
 }
 

@@ -497,133 +497,124 @@ __device__ __forceinline__ uint8_t *qf_place(const mm_mla_qfrag_args &a, int b, 
     const size_t r = (size_t)b * a.NH + h;
     return (uint8_t *)a.qf + (r >> 5) * MM_MLA_QF_TILE + 512 * piece + 16 * (r & 31);
 }
-/* One wave: latents e0 .. e0 + 32 S - 1 of head h for NX x 16 positions (b[x]:
- * lane % 16's of the x-th); ph / pl[s][x] piece e0 / 8 + 4 s + lane / 16. */
-template <int NX, int S>
-__device__ __forceinline__ void qf_wave(const mm_mla_qfrag_args &a, int h, const int (&b)[NX], int e0, i32x4 (&ph)[S][NX], i32x4 (&pl)[S][NX]) {
+/* One wave: latents e0 .. e0 + 31 of head h for 16 positions from b0 on (past the
+ * last: that again); ph / pl piece e0 / 8 + lane / 16 of position b0 + lane % 16.
+ *
+ * Both operands come through LDS (`buf`, the wave's own), WIN windows of 64 at a
+ * time: a load whose neighbouring lanes are in different rows costs the L1 a
+ * request per lane, and the fragments read from memory that way took 10 of 19 us
+ * (512 positions of 16 heads).  Rows are 16-byte pieces, W's 8 of them and q's 16;
+ * piece p of row r lies in slot p ^ qf_swz(r) or p ^ r, so that the 16 rows of a
+ * fragment fall on all banks. */
+#define QF_WINDOW 8192
+__device__ __forceinline__ int qf_swz(int r) { return (r >> 3 & 3) << 1 | (r >> 1 & 1); }
+template <int WIN>
+__device__ __forceinline__ void qf_wave(const mm_mla_qfrag_args &a, int h, int b0, int e0, uint8_t *buf, i32x4 &ph, i32x4 &pl) {
     const int lane = threadIdx.x & 63, n16 = lane & 15, g = lane >> 4;
-    const uint16_t *wr = a.wukT + ((size_t)h * KVL + e0 + 8 * (n16 >> 2) + (n16 & 3)) * a.QKN + 8 * g;
-    const float *qr[NX];
+    const uint16_t *wr = a.wukT + ((size_t)h * KVL + e0 + (lane >> 3)) * a.QKN;
+    f32x4 y[2] = {};
+    for (int k0 = 0; k0 < a.QKN; k0 += 64 * WIN) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   /* the windows before are read */
 #pragma unroll
-    for (int x = 0; x < NX; x++) qr[x] = a.q + ((size_t)b[x] * a.NH + h) * (a.QKN + MM_MLA_QKR) + 8 * g;
-    f32x4 y[S][NX][2] = {};
-    constexpr int GB = S * NX > 2 ? 2 : 4;             /* 32-wide steps whose loads are in flight */
-    for (int k0 = 0; k0 < a.QKN; k0 += 32 * GB) {
-        i32x4 wv[GB][S][2];
-        f32x4 xv[GB][NX][2];
+        for (int u = 0; u < WIN; u++) {
+            const int k = k0 + 64 * u;
+            if (k >= a.QKN) break;                     /* uniform */
+            uint8_t *p = buf + u * QF_WINDOW;
 #pragma unroll
-        for (int u = 0; u < GB; u++) {
-            const int k = min(k0 + 32 * u, a.QKN - 32);
+            for (int i = 0; i < 4; i++)                /* 8 rows of W (a last half window: its end again) */
+                lds_dma16(wr + 8 * i * a.QKN + min(k + 8 * ((lane & 7) ^ qf_swz(8 * i + (lane >> 3))), a.QKN - 8), p + 1024 * i);
 #pragma unroll
-            for (int s = 0; s < S; s++) {
-                wv[u][s][0] = *(const i32x4 *)(wr + 32 * s * a.QKN + k);
-                wv[u][s][1] = *(const i32x4 *)(wr + (32 * s + 4) * a.QKN + k);
-            }
-#pragma unroll
-            for (int x = 0; x < NX; x++) {
-                xv[u][x][0] = *(const f32x4 *)(qr[x] + k);
-                xv[u][x][1] = *(const f32x4 *)(qr[x] + k + 4);
+            for (int i = 0; i < 4; i++) {              /* 4 rows of q (a last half window: into q_pe) */
+                const int r = 4 * i + g;
+                lds_dma16(a.q + ((size_t)min(b0 + r, a.R - 1) * a.NH + h) * (a.QKN + MM_MLA_QKR) + k + 4 * (n16 ^ r), p + 4096 + 1024 * i);
             }
         }
-        __builtin_amdgcn_sched_barrier(0);             /* (the loads sink to their uses otherwise, one at a time) */
+        VMCNT_WAIT(0);
+        asm volatile("" ::: "memory");
 #pragma unroll
-        for (int u = 0; u < GB; u++) {
+        for (int u = 0; u < 2 * WIN; u++) {
             if (k0 + 32 * u >= a.QKN) break;
+            const uint8_t *p = buf + (u >> 1) * QF_WINDOW, *qp = p + 4096 + 256 * n16;
+            const int c = 8 * (u & 1) + 2 * g;
+            i32x4 xh, xl;
+            qf_split(*(const f32x4 *)(qp + 16 * (c ^ n16)), *(const f32x4 *)(qp + 16 * ((c + 1) ^ n16)), 1.0f, xh, xl);
 #pragma unroll
-            for (int x = 0; x < NX; x++) {
-                i32x4 xh, xl;
-                qf_split(xv[u][x][0], xv[u][x][1], 1.0f, xh, xl);
-#pragma unroll
-                for (int s = 0; s < S; s++)
-#pragma unroll
-                    for (int t = 0; t < 2; t++) {
-                        y[s][x][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wv[u][s][t]), __builtin_bit_cast(bf16x8, xh), y[s][x][t], 0, 0, 0);
-                        y[s][x][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wv[u][s][t]), __builtin_bit_cast(bf16x8, xl), y[s][x][t], 0, 0, 0);
-                    }
+            for (int t = 0; t < 2; t++) {
+                const int r = 8 * (n16 >> 2) + (n16 & 3) + 4 * t;
+                const i32x4 wv = *(const i32x4 *)(p + 128 * r + 16 * ((g + 4 * (u & 1)) ^ qf_swz(r)));
+                y[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wv), __builtin_bit_cast(bf16x8, xh), y[t], 0, 0, 0);
+                y[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wv), __builtin_bit_cast(bf16x8, xl), y[t], 0, 0, 0);
             }
         }
     }
-#pragma unroll
-    for (int s = 0; s < S; s++)
-#pragma unroll
-        for (int x = 0; x < NX; x++) qf_split(y[s][x][0], y[s][x][1], a.scale2, ph[s][x], pl[s][x]);
+    qf_split(y[0], y[1], a.scale2, ph, pl);
 }
 
 /* Few positions: grid (KVL / 64 slabs and one for q_pe, NH, ceil(R / 32)), wave w
  * latents 32 (w % 2) .. + 31 of the slab for positions 16 (w / 2) .. + 15. */
 extern "C" __global__ __launch_bounds__(256) void mm_mla_qfrag(mm_mla_qfrag_args a) {
+    __shared__ __attribute__((aligned(1024))) uint8_t qbuf[4][2 * QF_WINDOW];
     const int slab = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    i32x4 ph[1][1], pl[1][1];
+    i32x4 ph, pl;
     int b, piece;
     if (slab == KVL / 64) {                            /* q_pe: a piece per thread */
         b = blockIdx.z * 32 + (tid >> 3);
         piece = KVL / 8 + (tid & 7);
         const float *q = a.q + ((size_t)min(b, a.R - 1) * a.NH + h) * (a.QKN + MM_MLA_QKR) + a.QKN + 8 * (tid & 7);
-        qf_split(*(const f32x4 *)q, *(const f32x4 *)(q + 4), a.scale2, ph[0][0], pl[0][0]);
+        qf_split(*(const f32x4 *)q, *(const f32x4 *)(q + 4), a.scale2, ph, pl);
     } else {
-        const int e0 = 64 * slab + 32 * (w & 1);
-        b = blockIdx.z * 32 + 16 * (w >> 1) + (lane & 15);
+        const int e0 = 64 * slab + 32 * (w & 1), b0 = blockIdx.z * 32 + 16 * (w >> 1);
+        b = b0 + (lane & 15);
         piece = e0 / 8 + (lane >> 4);
-        const int bc[1] = {min(b, a.R - 1)};
-        qf_wave<1, 1>(a, h, bc, e0, ph, pl);
+        qf_wave<2>(a, h, b0, e0, qbuf[w], ph, pl);
     }
     if (b >= a.R) return;
     uint8_t *p = qf_place(a, b, h, piece);
-    *(i32x4 *)p = ph[0][0];
-    *(i32x4 *)(p + MM_MLA_QF_TILE / 2) = pl[0][0];
+    *(i32x4 *)p = ph;
+    *(i32x4 *)(p + MM_MLA_QF_TILE / 2) = pl;
 }
 
 /* More: a block of eight heads (wave w head w), whose 16-byte pieces are one line
- * and leave together through LDS; 16 NX positions and 32 S latents per wave.  A
- * wave's reads are 16 rows of 64 bytes each and set the time, so that many
- * positions take a larger tile (512 of 16 heads, NX x S = 1 x 1 22 us).  grid (KVL
- * / (32 S) and one for q_pe, ceil(NH / 8), ceil(R / (16 NX))). */
-template <int NX, int S>
-__device__ __forceinline__ void qf_block(const mm_mla_qfrag_args &a) {
-    __shared__ __attribute__((aligned(16))) i32x4 st[2][4][16 * NX][8];   /* [hi, lo][piece][position][head] */
-    const int slab = blockIdx.x, h0 = blockIdx.y * 8, b0 = blockIdx.z * 16 * NX;
+ * and leave together through LDS; 32 latents of 16 positions.  One window at a time,
+ * so that a CU holds two blocks (512 of 16 heads 15.5 us; two windows 20.4, more
+ * positions or latents per block 19).  grid (KVL / 32 and one for q_pe, ceil(NH /
+ * 8), ceil(R / 16)). */
+extern "C" __global__ __launch_bounds__(512) void mm_mla_qfrag_8(mm_mla_qfrag_args a) {
+    __shared__ __attribute__((aligned(1024))) uint8_t qbuf[8][QF_WINDOW];
+    typedef i32x4 pieces[2][4][16][8];                 /* [hi, lo][piece][position][head], over the windows */
+    static_assert(sizeof(pieces) <= sizeof(qbuf), "a block's pieces");
+    pieces &st = *(pieces *)(void *)qbuf;
+    const int slab = blockIdx.x, h0 = blockIdx.y * 8, b0 = blockIdx.z * 16;
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int sh = tid & 7, sb = tid >> 3 & 15, sp = tid >> 7;
-    if (slab == KVL / (32 * S)) {                      /* q_pe: 8 pieces, 16 NX positions, 8 heads */
+    if (slab == KVL / 32) {                            /* q_pe: 8 pieces, 16 positions, 8 heads */
+        if (b0 + sb >= a.R || h0 + sh >= a.NH) return;
+        const float *q = a.q + ((size_t)(b0 + sb) * a.NH + h0 + sh) * (a.QKN + MM_MLA_QKR) + a.QKN;
 #pragma unroll
-        for (int u = 0; u < 2 * NX; u++) {
-            const int b = b0 + 16 * (u >> 1) + sb, piece = sp + 4 * (u & 1);
-            if (b >= a.R || h0 + sh >= a.NH) continue;
-            const float *q = a.q + ((size_t)b * a.NH + h0 + sh) * (a.QKN + MM_MLA_QKR) + a.QKN + 8 * piece;
+        for (int u = 0; u < 2; u++) {
+            const int piece = sp + 4 * u;
             i32x4 ph, pl;
-            qf_split(*(const f32x4 *)q, *(const f32x4 *)(q + 4), a.scale2, ph, pl);
-            uint8_t *p = qf_place(a, b, h0 + sh, KVL / 8 + piece);
+            qf_split(*(const f32x4 *)(q + 8 * piece), *(const f32x4 *)(q + 8 * piece + 4), a.scale2, ph, pl);
+            uint8_t *p = qf_place(a, b0 + sb, h0 + sh, KVL / 8 + piece);
             *(i32x4 *)p = ph;
             *(i32x4 *)(p + MM_MLA_QF_TILE / 2) = pl;
         }
         return;
     }
-    i32x4 ph[S][NX], pl[S][NX];
-    int b[NX];
-#pragma unroll
-    for (int x = 0; x < NX; x++) b[x] = min(b0 + 16 * x + (lane & 15), a.R - 1);
-    qf_wave<NX, S>(a, min(h0 + w, a.NH - 1), b, 32 * S * slab, ph, pl);
-#pragma unroll
-    for (int s = 0; s < S; s++) {
-        if (s) __syncthreads();                        /* the pieces before are read */
-#pragma unroll
-        for (int x = 0; x < NX; x++) {
-            st[0][lane >> 4][16 * x + (lane & 15)][w] = ph[s][x];
-            st[1][lane >> 4][16 * x + (lane & 15)][w] = pl[s][x];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int x = 0; x < NX; x++)
-#pragma unroll
-            for (int u = 0; u < 2; u++)
-                if (b0 + 16 * x + sb < a.R && h0 + sh < a.NH)
-                    *(i32x4 *)(qf_place(a, b0 + 16 * x + sb, h0 + sh, 4 * (S * slab + s) + sp) + u * (MM_MLA_QF_TILE / 2)) = st[u][sp][16 * x + sb][sh];
+    i32x4 ph, pl;
+    qf_wave<1>(a, min(h0 + w, a.NH - 1), b0, 32 * slab, qbuf[w], ph, pl);
+    __syncthreads();                                   /* the windows are read */
+    st[0][lane >> 4][lane & 15][w] = ph;
+    st[1][lane >> 4][lane & 15][w] = pl;
+    __syncthreads();
+    if (b0 + sb < a.R && h0 + sh < a.NH) {
+        uint8_t *p = qf_place(a, b0 + sb, h0 + sh, 4 * slab + sp);
+        *(i32x4 *)p = st[0][sp][sb][sh];
+        *(i32x4 *)(p + MM_MLA_QF_TILE / 2) = st[1][sp][sb][sh];
     }
 }
-extern "C" __global__ __launch_bounds__(512) void mm_mla_qfrag_8(mm_mla_qfrag_args a) { qf_block<1, 1>(a); }
-extern "C" __global__ __launch_bounds__(512) void mm_mla_qfrag_w(mm_mla_qfrag_args a) { qf_block<MM_MLA_QF_NX, MM_MLA_QF_S>(a); }
 
 /* A shared prefix, and one position per sequence over its own keys. */
 extern "C" __global__ __launch_bounds__(512, 2) void mm_mla_attn_tiles(mm_mla_tiles_args a) { tl_block<false>(a); }
@@ -654,13 +645,12 @@ __device__ __forceinline__ void merge_uv(const mm_mla_merge_uv_args &a) {
     const int ct0 = sp * per, ct1 = min(ct0 + per, ncol);
     const int n16 = lane & 15, kq = 8 * (lane >> 4);
     typedef const __attribute__((address_space(1))) i32x4 *glb_c4;
-    const uint16_t *wuv = a.kv_b + ((size_t)h * (a.QKN + a.VHD) + a.QKN) * KVL;
     /* this wave's first column tile's weights: in flight during the merge */
     i32x4 wv[KVL / 32];
     auto weights = [&](int ct) {
-        const uint16_t *p = wuv + (size_t)min(16 * ct + n16, a.VHD - 1) * KVL + kq;
+        const uint16_t *p = a.wuvf + ((size_t)h * ncol + ct) * MM_MLA_UVF_TILE + 8 * lane;
 #pragma unroll
-        for (int s = 0; s < KVL / 32; s++) wv[s] = *(glb_c4)(uintptr_t)(p + 32 * s);
+        for (int s = 0; s < KVL / 32; s++) wv[s] = *(glb_c4)(uintptr_t)(p + 512 * s);
     };
     weights(min(ct0 + w, ncol - 1));
 
