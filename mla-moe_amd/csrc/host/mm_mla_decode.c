@@ -122,6 +122,8 @@ static int decode_run(mm_ctx *c, int layer, const decode_plan *p, const float *q
     mm_mla_qfrag_args qa = {q, wukT, qf, R, NH, QKN,
                             g->softmax_scale * 1.44269504088896341f};
     int st;
+    /* (4 positions of 16 heads: 3.4 us, in blocks of eight heads 4.3; 39 of 20: 5.9
+     * both; 48 of 16: 4.9, 4.6) */
     if (R < 48)
         st = mm_launch(c, K_MLA_QFRAG, MM_MLA_KVL / 64 + 1, (unsigned)NH, (unsigned)(R + 31) / 32, 256, 0, &qa);
     else
@@ -137,11 +139,11 @@ static int decode_run(mm_ctx *c, int layer, const decode_plan *p, const float *q
         const size_t h0 = (size_t)r0 * NH;
         if ((st = attend(c, p, k, qf, r0, n, ml, po))) return st;
         /* blocks of the merge: four waves a position each, a column tile each, for
-         * few positions (4 of 16 heads 7.5 us, with eight waves 10; 16: 8.8, 10.4);
-         * eight waves for more, 4 positions per block as long as every CU has at
-         * most one block, else 8 (64 positions: 10.2, with four waves 11.4; 39 of
-         * 20 heads and 256 columns: 10.6, 11.6); from 256 positions on 16 per block
-         * and a head's columns together (512: 18.3, with eight waves 20.7) */
+         * few positions (4 of 16 heads 5.6 us, with eight waves 6.7); eight waves for
+         * more, 4 positions per block as long as every CU has at most one block,
+         * else 8 (64 positions: 8.1, with four waves 8.6; 39 of 20 heads and 256
+         * columns: 7.8, 4 per block 10.7); from 256 positions on 16 per block and a
+         * head's columns together (512: 12.9, 8 per block 17.0, with eight waves 13.4) */
         const int ncol = (VHD + 15) / 16, nw = R <= 16 || R >= 256 ? 4 : 8;
         const int split = R >= 256 ? 1 : (ncol + nw - 1) / nw;
         int ppb = R >= 256 ? 16 : 4, wpp = 1;
