@@ -272,6 +272,23 @@ def test_few_rows_in_groups(monkeypatch, NH, B):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("NH,B,QKN,VHD", [(5, 3, 96, 24), (20, 50, 96, 40), (9, 60, 160, 272), (16, 49, 32, 16), (3, 260, 224, 100)])
+def test_prefix_query_layouts(NH, B, QKN, VHD):
+    """Query dimensions that end inside a window of 64, few and many positions,
+    heads that do not fill a block."""
+    prefix_case(NH, B, 70, 9, [b % 10 for b in range(B)], QKN, VHD, seed=300 + NH)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("NH,B,rows,L,sinks,window,lens", [
+    (16, 2, 20, 7, 2, 5, [7, 3]), (1, 1, 150, 200, 3, 40, None), (1, 3, 70, 65, 0, 1, [65, 64, 1]),
+    (128, 1, 2, 33, 1, 16, None), (16, 1, 1, 1, 0, 1, None), (6, 2, 25, 90, 90, 3, [90, 31])])
+def test_window_odd_shapes(NH, B, rows, L, sinks, window, lens):
+    """More rows than keys, one head (64 positions a tile), many heads, a single key."""
+    window_case(NH, B, rows, L, sinks, window, lens, 64, 48, seed=400 + NH + rows)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("bad", [0x7FC0, 0x7F80, 0xFF80])
 def test_window_keys_that_are_not_finite(bad):
     """A drafted position whose cache row is not finite: the rows before it,
