@@ -83,6 +83,28 @@ __device__ __forceinline__ void tl_scores(const i32x4 (&qh)[18], const i32x4 (&q
     }
 }
 
+/* Which of a tile's 32 keys hold a value that is not finite (bit r: row r of its
+ * three parts in LDS): lane l has half l / 32 of row l % 32, in slots of 16 bytes
+ * in whatever order. */
+__device__ __forceinline__ uint32_t tl_not_finite(uint32_t r0, uint32_t r1, uint32_t kp) {
+    const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5;
+    uint32_t top = 0;
+    auto look = [&](uint32_t p, int n) {
+#pragma unroll 1
+        for (int i = 0; i < n; i++) {
+            const i32x4 x = *(lds_w4)(uintptr_t)(p + 16 * i);
+            /* two bf16 each: an exponent of ones carries into the sign's place */
+#pragma unroll
+            for (int k = 0; k < 4; k++) top |= ((uint32_t)x[k] & 0x7f807f80u) + 0x00800080u;
+        }
+    };
+    look(r0 + (uint32_t)(row * 576 + half * 288), 18);
+    look(r1 + (uint32_t)(row * 448 + half * 224), 14);
+    look(kp + (uint32_t)(row * 128 + half * 64), 4);
+    const uint64_t m = __builtin_amdgcn_ballot_w64((top & 0x80008000u) != 0);
+    return (uint32_t)m | (uint32_t)(m >> 32);
+}
+
 /* A block's rows and keys. */
 struct tl_job {
     const uint16_t *keys;          /* first of the chunk's keys; WIN: the sequence's cache */
@@ -413,7 +435,7 @@ __device__ __forceinline__ void tl_block(const mm_mla_tiles_args &a) {
         }
         float mx = -INFINITY;
         if (!all) {
-            uint32_t own = 0;                          /* this lane's keys that are not finite */
+            bool some = false;                         /* a score that is not finite: of such a key, or such a query */
 #pragma unroll
             for (int i = 0; i < 16; i++) {
                 const int v = 32 * t + 8 * (i >> 2) + 4 * hi + (i & 3);
@@ -422,16 +444,14 @@ __device__ __forceinline__ void tl_block(const mm_mla_tiles_args &a) {
                     const int key = tl_key(a, j, j.v0 + v);
                     const bool nf = see && !(fabsf(s1[i]) < INFINITY);
                     see = see && key <= pos && (key < a.sinks || key > pos - a.window);
-                    own |= nf ? 1u << (8 * (i >> 2) + 4 * hi + (i & 3)) : 0u;
+                    some |= nf;
                     if (nf) s1[i] = __builtin_nanf("");
                 }
                 if (!see) s1[i] = -INFINITY;
             }
-            if (WIN && __builtin_amdgcn_ballot_w64(own != 0)) {
-                bad = own;
-#pragma unroll
-                for (int off = 1; off < MM_WAVE; off <<= 1) bad |= (uint32_t)__shfl_xor((int)bad, off, MM_WAVE);
-            }
+            /* every row's score of a key that is not finite is not, so both halves'
+             * waves find the same; all of the tile is in LDS until its output step */
+            if (WIN && __builtin_amdgcn_ballot_w64(some)) bad = tl_not_finite(lds0 + (uint32_t)(t & 3) * TL_R0, lds0 + TL_O1 + d, lds0 + TL_OK + dk);
         }
 #pragma unroll
         for (int i = 0; i < 16; i++) mx = fmaxf(mx, s1[i]);

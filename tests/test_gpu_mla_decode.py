@@ -451,3 +451,64 @@ def test_refusals_without_a_gpu():
     assert L.mm_mla_window_decode_dev(None, 0, 1, 1, None, None, 1, None, 1, 0, 1, None, None, 0) == -1
     assert L.mm_mla_prefix_decode_workspace(None, 1, 1, 1, C.byref(b)) == -1 and b.value == 0
     assert L.mm_mla_window_decode_workspace(None, 1, 1, 1, 1, 1, None) == -1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("NH,rows,head,row,what", [
+    (16, 1, 5, 0, "nope"), (16, 9, 0, 4, "nope"), (16, 9, 15, 8, "rope"), (20, 7, 19, 0, "rope"), (3, 4, 1, 2, "nope"),
+    (16, 9, 3, 5, "inf"), (16, 1, 15, 0, "large"), (20, 7, 2, 3, "large")])
+def test_window_query_that_is_not_finite(NH, rows, head, row, what):
+    """One head's query of one position is not finite, or so large that scores
+    overflow: every other head and position has its own result."""
+    B, L, sinks, window = 2, 300, 2, 70
+    rng = np.random.default_rng(46)
+    q = synth.normal_f32(rng, (B, rows, NH, 192), 2.0)
+    cache = synth.normal_bf16(rng, (B, L, KVL + QKR), 1.0)
+    if what == "nope":
+        q[0, row, head, 7] = np.nan
+    elif what == "rope":
+        q[0, row, head, 150] = np.nan
+    elif what == "inf":
+        q[0, row, head, 128:130] = np.inf, -np.inf
+    else:
+        q[0, row, head, 128:] = 3e38
+    ctx, kv_b = loaded(NH)
+    with ctx:
+        got = ctx.mla_window_decode(0, q, cache, sinks, window)
+    got = got.reshape(B, rows, NH, 128)
+    at = np.arange(L)
+    for b in range(B):
+        for r in range(rows):
+            p = L - rows + r
+            keys = f64(cache[b, at[(at <= p) & ((at < sinks) | (at > p - window))]])
+            for h in range(NH):
+                if (b, r, h) == (0, row, head):
+                    assert what == "large" or not np.isfinite(got[b, r, h]).any()
+                    continue
+                w = kv_b.reshape(NH, 256, KVL)[h]
+                close(got[b, r, h:h + 1], attend(q[b, r, h:h + 1].astype(np.float64), w, keys, 1, 128, 128), (b, r, h))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("NH,rows,bad", [(16, 9, 5), (20, 5, 4), (16, 2, 1), (3, 8, 3), (16, 40, 17)])
+def test_window_position_that_is_not_finite(NH, rows, bad):
+    """A drafted or prompt position whose hidden state was not finite: neither is
+    its query nor its cache row.  The positions before it do not see it, and are
+    what they are without it; those from it on have no finite value."""
+    B, L, sinks, window = 2, 300, 2, 70
+    rng = np.random.default_rng(47)
+    q = synth.normal_f32(rng, (B, rows, NH, 192), 2.0)
+    cache = synth.normal_bf16(rng, (B, L, KVL + QKR), 1.0)
+    clean, at = cache.copy(), np.arange(L)
+    q[1, bad], cache[1, L - rows + bad] = np.nan, NAN16
+    ctx, kv_b = loaded(NH)
+    with ctx:
+        got = ctx.mla_window_decode(0, q, cache, sinks, window)
+    for b in range(B):
+        for r in range(rows):
+            if b == 1 and r >= bad:
+                assert not np.isfinite(got[b, r]).any(), (b, r)
+                continue
+            p = L - rows + r
+            keys = f64(clean[b, at[(at <= p) & ((at < sinks) | (at > p - window))]])
+            close(got[b, r].reshape(NH, 128), attend(q[b, r].astype(np.float64), kv_b, keys, NH, 128, 128), (b, r))
