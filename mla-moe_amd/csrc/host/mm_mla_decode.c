@@ -179,7 +179,7 @@ int mm_mla_prefix_decode_workspace(mm_ctx *c, int B, int prefix_len, int kv_len,
     if (!bytes) return mm_fail(MM_ERR_INVALID, "mm_mla_prefix_decode_workspace: NULL argument");
     *bytes = 0;
     const int st = prefix_check(c, "mm_mla_prefix_decode_workspace", B, prefix_len, kv_len);
-    if (st || B == 0) return st;
+    if (st || B == 0 || prefix_len + kv_len == 0) return st;
     const decode_keys k = prefix_keys(NULL, prefix_len, NULL, kv_len, NULL, kv_len);
     decode_plan p;
     plan_decode(c, B, &k, &p);
@@ -203,6 +203,10 @@ int mm_mla_prefix_decode_dev(mm_ctx *c, int layer, int B, const float *q, const 
     if ((prefix_len && (uintptr_t)prefix % 16) || (kv_len && (uintptr_t)cache % 16) || (uintptr_t)q % 16)
         return mm_fail(MM_ERR_INVALID, "%s: q, prefix and cache must be 16-byte aligned", name);
     if ((st = mm_set_device(c))) return st;
+    if (prefix_len + kv_len == 0) {                   /* no chunk to merge */
+        mm_zero32_args za = {(uint32_t *)ctx_out, (uint64_t)B * c->mla.n_heads * c->mla.v_head_dim};
+        return mm_launch(c, K_ZERO32, 256, 1, 1, 256, 0, &za);
+    }
     const decode_keys k = prefix_keys(prefix, prefix_len, cache, seq_stride, kv_lens, kv_len);
     decode_plan p;
     plan_decode(c, B, &k, &p);

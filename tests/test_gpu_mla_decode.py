@@ -512,3 +512,23 @@ def test_window_position_that_is_not_finite(NH, rows, bad):
             p = L - rows + r
             keys = f64(clean[b, at[(at <= p) & ((at < sinks) | (at > p - window))]])
             close(got[b, r].reshape(NH, 128), attend(q[b, r].astype(np.float64), kv_b, keys, NH, 128, 128), (b, r))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("NH,B,VHD", [(16, 3, 128), (3, 40, 24), (128, 1, 16)])
+def test_no_keys_at_all(NH, B, VHD):
+    """No prefix and no own row: zeros without a workspace, captured too, and
+    nothing behind the last row."""
+    ctx, _ = loaded(NH, 64, VHD)
+    with ctx:
+        assert ctx.mla_prefix_decode_workspace(B, 0, 0) == 0
+        q = ctx.to_device(np.full((B, NH, 64 + QKR), np.nan, np.float32))
+        outs = [ctx.to_device(np.full((B + 1, NH * VHD), 7.0, np.float32)) for _ in range(2)]
+        ctx.mla_prefix_decode_dev(0, B, q, None, 0, None, 0, 0, outs[0])
+        g = Graph(ctx, lambda: ctx.mla_prefix_decode_dev(0, B, q, None, 0, None, 0, 0, outs[1]))
+        for _ in range(3):
+            g.replay()
+        for o in outs:
+            got = o.download()
+            assert np.all(got[:B] == 0.0) and np.all(got[B] == 7.0)
+        g.close()
