@@ -31,7 +31,7 @@ typedef struct {
     int R, HG;
     int pchunk, np;                /* the prefix: keys per chunk, chunks */
     int ochunk, no;                /* own keys */
-    int G;                         /* rows whose partials are held at once */
+    int G;                         /* rows whose queries and partials are held at once */
     size_t o_ml, o_po, bytes;      /* (the queries at 0) */
 } decode_plan;
 
@@ -84,14 +84,16 @@ static void plan_decode(const mm_ctx *c, int R, const decode_keys *k, decode_pla
     tiles_chunks(R, NH, k->rows, k->prefix_len, k->own, p);
     int unit = 1;                  /* rows that fill whole tiles */
     while ((unit * NH) % 64) unit++;
-    const size_t row = (size_t)p->HG * (p->np + p->no) * (16 * MM_MLA_KVL + 32) * 4;
+    const size_t row = (size_t)p->HG * (p->np + p->no) * (16 * MM_MLA_KVL + 32) * 4 +
+                       (size_t)NH * (MM_MLA_QF_TILE / 32);
     p->G = R;
-    if (row && (size_t)R * row > c->mla_part_max) {
+    if ((size_t)R * row > c->mla_part_max) {
         const size_t g = c->mla_part_max / row / unit * unit;
         p->G = g > 0 ? (int)g : unit;
+        if (p->G > R) p->G = R;
     }
-    p->o_ml = ((size_t)R * NH + 31) / 32 * MM_MLA_QF_TILE;
-    const size_t parts = (size_t)(p->G < R ? p->G : R) * p->HG * (p->np + p->no);
+    p->o_ml = ((size_t)p->G * NH + 31) / 32 * MM_MLA_QF_TILE;
+    const size_t parts = (size_t)p->G * p->HG * (p->np + p->no);
     p->o_po = p->o_ml + al256(parts * 32 * 4);
     p->bytes = p->o_po + al256(parts * 16 * MM_MLA_KVL * 4);
 }
@@ -102,7 +104,7 @@ static int attend(mm_ctx *c, const decode_plan *p, const decode_keys *k, const u
                   float *ml, float *po) {
     const mm_mla_config *g = &c->mla;
     const int NH = g->n_heads, M = n * NH, rows = n < k->rows ? n : k->rows, nseq = n / rows;
-    mm_mla_tiles_args a = {qf, r0 * NH, ml, po, M, NH, p->HG, p->np + p->no,
+    mm_mla_tiles_args a = {qf, ml, po, M, NH, p->HG, p->np + p->no,
                            k->prefix, k->prefix_len, p->pchunk, p->np, k->cache, k->kv_lens, k->kv_len, k->seq_stride,
                            r0 / k->rows, nseq, rows, p->ochunk, p->no, k->rows, r0 % k->rows, k->sinks, k->window};
     const unsigned np = (unsigned)((M + 63) / 64) * (unsigned)p->np;
@@ -119,16 +121,7 @@ static int decode_run(mm_ctx *c, int layer, const decode_plan *p, const float *q
     float *ml = (float *)(ws + p->o_ml), *po = (float *)(ws + p->o_po);
     const uint16_t *wukT = c->mla_kvb[layer] + (size_t)NH * (QKN + VHD) * MM_MLA_KVL;
     const uint16_t *wuvf = wukT + (size_t)NH * MM_MLA_KVL * QKN;
-    mm_mla_qfrag_args qa = {q, wukT, qf, R, NH, QKN,
-                            g->softmax_scale * 1.44269504088896341f};
     int st;
-    /* (4 positions of 16 heads: 3.4 us, in blocks of eight heads 4.3; 39 of 20: 5.9
-     * both; 48 of 16: 4.9, 4.6) */
-    if (R < 48)
-        st = mm_launch(c, K_MLA_QFRAG, MM_MLA_KVL / 64 + 1, (unsigned)NH, (unsigned)(R + 31) / 32, 256, 0, &qa);
-    else
-        st = mm_launch(c, K_MLA_QFRAG_8, MM_MLA_KVL / 32 + 1, (unsigned)(NH + 7) / 8, (unsigned)(R + 15) / 16, 512, 0, &qa);
-    if (st) return st;
     for (int r0 = 0, n; r0 < R; r0 += n) {
         n = R - r0 < p->G ? R - r0 : p->G;
         if (k->rows > 1 && n < R) {                   /* whole sequences, or within one */
@@ -137,6 +130,15 @@ static int decode_run(mm_ctx *c, int layer, const decode_plan *p, const float *q
             else if (n > left) n = left;
         }
         const size_t h0 = (size_t)r0 * NH;
+        mm_mla_qfrag_args qa = {q + h0 * (QKN + MM_MLA_QKR), wukT, qf, n, NH, QKN,
+                                g->softmax_scale * 1.44269504088896341f};
+        /* by the call's rows, as below (4 positions of 16 heads: 3.4 us, in blocks of
+         * eight heads 4.3; 39 of 20: 5.9 both; 48 of 16: 4.9, 4.6) */
+        if (R < 48)
+            st = mm_launch(c, K_MLA_QFRAG, MM_MLA_KVL / 64 + 1, (unsigned)NH, (unsigned)(n + 31) / 32, 256, 0, &qa);
+        else
+            st = mm_launch(c, K_MLA_QFRAG_8, MM_MLA_KVL / 32 + 1, (unsigned)(NH + 7) / 8, (unsigned)(n + 15) / 16, 512, 0, &qa);
+        if (st) return st;
         if ((st = attend(c, p, k, qf, r0, n, ml, po))) return st;
         /* blocks of the merge: four waves a position each, a column tile each, for
          * few positions (4 of 16 heads 5.6 us, with eight waves 6.7); eight waves for

@@ -500,8 +500,7 @@ typedef struct {
     float scale2;             /* softmax scale / ln 2, taken into the queries */
 } mm_mla_qfrag_args;
 typedef struct {
-    const uint16_t *qf;       /* the call's queries (mm_mla_qfrag) */
-    int row0;                 /* the launch's first row among them */
+    const uint16_t *qf;       /* the launch's queries (mm_mla_qfrag) */
     float *part_ml;           /* [M / NH, HG, pchunks, 2, 16] */
     float *part_o;            /* [M / NH, HG, pchunks, 16, KVL] */
     int M, NH, HG, pchunks;

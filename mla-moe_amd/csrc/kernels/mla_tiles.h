@@ -108,7 +108,7 @@ __device__ __forceinline__ uint32_t tl_not_finite(uint32_t r0, uint32_t r1, uint
 /* A block's rows and keys. */
 struct tl_job {
     const uint16_t *keys;          /* first of the chunk's keys; WIN: the sequence's cache */
-    int row0, nrows;               /* flat rows (position, head) of the call */
+    int row0, nrows;               /* flat rows (position, head) of the launch */
     int chunk;                     /* its place among a row's partials */
     int nk;                        /* keys of the chunk */
     /* WIN: the chunk's key v is key v0 + v of the tile's list: the sinks, then
@@ -373,7 +373,7 @@ __device__ __forceinline__ void tl_block(const mm_mla_tiles_args &a) {
     }
     i32x4 qh[18], ql[18];
     {
-        const int row = a.row0 + j.row0 + min(32 * rh + c32, j.nrows - 1);
+        const int row = j.row0 + min(32 * rh + c32, j.nrows - 1);
         const uint8_t *p = (const uint8_t *)a.qf + (size_t)(row >> 5) * MM_MLA_QF_TILE + (36 * second + hi) * 512 + 16 * (row & 31);
 #pragma unroll
         for (int s = 0; s < 18; s++) {

@@ -532,3 +532,34 @@ def test_no_keys_at_all(NH, B, VHD):
             got = o.download()
             assert np.all(got[:B] == 0.0) and np.all(got[B] == 7.0)
         g.close()
+
+
+@pytest.mark.gpu
+def test_workspace_stays_within_the_cap(monkeypatch):
+    """Queries and partials of the rows in flight together, however many rows."""
+    for cap in (None, 1 << 28):
+        if cap:
+            monkeypatch.setenv("MLAMOE_MLA_PART_MAX", str(cap))
+        for NH in (16, 20, 3):
+            with mlamoe.Context(0) as ctx:
+                ctx.mla_init(NH, 128, QKR, KVL, 128)
+                most = (cap or 512 << 20) + 2304 * 32 + 512      # a last tile of queries, alignment
+                for rows in (1, 1000, 14600, 1 << 20):
+                    for p, own in ((4096, 0), (33, 7), (0, 1), (100000, 300)):
+                        assert 0 < ctx.mla_prefix_decode_workspace(rows, p, own) <= most, (cap, NH, rows, p, own)
+                    for n, w in ((8192, 4096), (50, 7)):
+                        assert 0 < ctx.mla_window_decode_workspace(1, rows, n, 4, w) <= most, (cap, NH, rows, n, w)
+                        assert 0 < ctx.mla_window_decode_workspace(rows, 1, n, 4, w) <= most, (cap, NH, rows, n, w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("NH,B,QKN,VHD", [(20, 130, 96, 40), (3, 300, 32, 16)])
+def test_many_rows_in_groups(monkeypatch, NH, B, QKN, VHD):
+    """As above with the query layout and merge of many rows, and lengths that
+    differ from sequence to sequence."""
+    lens = [(7 * b) % 51 for b in range(B)]
+    a = prefix_case(NH, B, 210, 50, lens, QKN, VHD, seed=500 + NH)
+    w = window_case(NH, 2, B // 2, 400, 5, 90, [400, 311], QKN, VHD, seed=501 + NH)
+    monkeypatch.setenv("MLAMOE_MLA_PART_MAX", str(9 << 20))
+    assert np.array_equal(a, prefix_case(NH, B, 210, 50, lens, QKN, VHD, seed=500 + NH))
+    assert np.array_equal(w, window_case(NH, 2, B // 2, 400, 5, 90, [400, 311], QKN, VHD, seed=501 + NH))
