@@ -14,6 +14,7 @@ import math
 import os
 import random
 import sys
+import weakref
 
 import torch
 
@@ -134,21 +135,32 @@ class _Dev:
         self.t, self.ptr, self.shape = t, t.data_ptr(), tuple(t.shape)
 
 
-_contexts = {}
-_LAYERS = 4096                    # a state's attention weights are a layer of its program's context
+_programs = {}
+_LAYERS = 256                     # a state's attention weights are a layer of its program
 
 
-def _context(heads):
-    """The program's context for one head geometry, its work on one stream:
-    [context, layers loaded, stream]."""
-    if heads not in _contexts:
+class _Program:
+    """A context for one head geometry, its work on one stream.  Its layers are
+    given back with it, when it has handed out all and no state of it is left."""
+
+    def __init__(self, heads):
         sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "mla-moe_amd"))
         import mlamoe
-        ctx, stream = mlamoe.Context(0), torch.cuda.Stream()
-        ctx.set_stream(stream.cuda_stream)
-        ctx.mla_init(heads, DIMS[heads][0], QKR, KVL, DIMS[heads][1], n_layers=_LAYERS)
-        _contexts[heads] = [ctx, 0, stream]
-    return _contexts[heads]
+        self.ctx, self.layers, self.stream = mlamoe.Context(0), 0, torch.cuda.Stream()
+        self.ctx.set_stream(self.stream.cuda_stream)
+        self.ctx.mla_init(heads, DIMS[heads][0], QKR, KVL, DIMS[heads][1], n_layers=_LAYERS)
+        weakref.finalize(self, _Program._close, self.ctx, self.stream).atexit = False
+
+    @staticmethod
+    def _close(ctx, stream):
+        stream.synchronize()
+        ctx.close()
+
+
+def _program(heads):
+    if heads not in _programs or _programs[heads].layers == _LAYERS:
+        _programs[heads] = _Program(heads)
+    return _programs[heads]
 
 
 def prepare(case, seed):
@@ -156,16 +168,16 @@ def prepare(case, seed):
     st = {"case": c, **_inputs(c, seed)}
     if own:
         torch.cuda.synchronize()
-        program = _context(c.get("heads", 16))
-        ctx = st["ctx"] = program[0]
+        program = st["program"] = _program(c.get("heads", 16))
+        ctx = st["ctx"] = program.ctx
         f32 = dict(dtype=torch.float32, device="cuda")
         if c["kind"] == "logprobs":
             t, k = c["rows"], c["top"]
             st["out"] = {"logprob": torch.zeros(t, **f32), "entropy": torch.zeros(t, **f32),
                          "top": torch.zeros((t, k), dtype=torch.int32, device="cuda"), "top_logprob": torch.zeros((t, k), **f32)}
         else:
-            st["layer"] = program[1]
-            program[1] += 1
+            st["layer"] = program.layers
+            program.layers += 1
             ctx.mla_load_layer(st["layer"], _Dev(st["kv_b"]), 4)          # 4: device pointers
             b, r, nh, _ = st["q"].shape
             st["out"] = torch.zeros((b, r, nh, DIMS[nh][1]), **f32)
