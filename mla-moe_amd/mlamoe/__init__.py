@@ -208,6 +208,14 @@ def _check(st):
         raise MMError(st, lib().mm_last_error().decode())
 
 
+def _shapes(what, **pairs):
+    """Refuses host arrays (value: array, the shape it needs) that a call would
+    read past."""
+    for name, (a, shape) in pairs.items():
+        if a is not None and np.shape(a) != shape:
+            raise MMError(-1, f"{what}: {name} has shape {np.shape(a)}, needs {shape}")
+
+
 class DevBuf:
     """A device allocation owned by a Context."""
 
@@ -575,6 +583,9 @@ class Context:
         lg = np.ascontiguousarray(logits, np.float32)
         T, stride = lg.shape
         n = stride if n is None else n
+        if n > stride:
+            raise MMError(-1, f"token_logprobs: n {n} > stride {stride}")
+        _shapes("token_logprobs", targets=(targets, (T,)))
         dl, de = self.to_device(lg), self.empty((T,), np.float32)
         dt = self.to_device(np.ascontiguousarray(targets, np.int32)) if targets is not None else None
         dp = self.empty((T,), np.float32) if targets is not None else None
@@ -666,6 +677,11 @@ class Context:
         """Host arrays: q [B, NH, QKN+QKR] fp32, prefix [P, KVL+QKR] and cache
         [B, L, KVL+QKR] bf16 (uint16), either None.  Returns ctx [B, NH*VHD]."""
         q = np.ascontiguousarray(q, np.float32)
+        g = self._mla_cfg
+        kvd = g.kv_lora_rank + g.qk_rope_head_dim
+        _shapes("mla_prefix_decode", q=(q, (len(q), g.n_heads, g.qk_nope_head_dim + g.qk_rope_head_dim)),
+                prefix=(prefix, (len(prefix) if prefix is not None else 0, kvd)),
+                cache=(cache, (len(q), np.shape(cache)[1] if np.ndim(cache) > 1 else 0, kvd)), kv_lens=(kv_lens, (len(q),)))
         up = lambda a, t: None if a is None else self.to_device(np.ascontiguousarray(a, t))  # noqa: E731
         dq, dp, dc, dl = up(q, np.float32), up(prefix, np.uint16), up(cache, np.uint16), up(kv_lens, np.int32)
         out = self.empty((q.shape[0], self._mla_cfg.n_heads * self._mla_cfg.v_head_dim), np.float32)
@@ -694,6 +710,10 @@ class Context:
         """Host arrays: q [B, rows, NH, QKN+QKR] fp32, cache [B, L, KVL+QKR]
         bf16 (uint16).  Returns ctx [B, rows, NH*VHD]."""
         q = np.ascontiguousarray(q, np.float32)
+        g = self._mla_cfg
+        _shapes("mla_window_decode", q=(q, (*q.shape[:2], g.n_heads, g.qk_nope_head_dim + g.qk_rope_head_dim)),
+                cache=(cache, (len(q), np.shape(cache)[1] if np.ndim(cache) > 1 else 0, g.kv_lora_rank + g.qk_rope_head_dim)),
+                kv_lens=(kv_lens, (len(q),)))
         dq, dc = self.to_device(q), self.to_device(np.ascontiguousarray(cache, np.uint16))
         dl = None if kv_lens is None else self.to_device(np.ascontiguousarray(kv_lens, np.int32))
         out = self.empty((*q.shape[:2], self._mla_cfg.n_heads * self._mla_cfg.v_head_dim), np.float32)

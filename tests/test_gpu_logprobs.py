@@ -280,3 +280,12 @@ def test_more_rows_than_a_grid_holds_are_refused():
     b = C.c_size_t(7)
     assert mlamoe.lib().mm_token_logprobs_workspace((1 << 23) + 1, 10, 1, C.byref(b)) == -2 and b.value == 0
     assert mlamoe.token_logprobs_workspace(1 << 23, 10, 1) == 0
+
+
+@pytest.mark.gpu
+def test_host_form_refuses_arrays_too_short(ctx):
+    x = np.zeros((3, 64), np.float32)
+    for call in (lambda: ctx.token_logprobs(x, [1, 2], 1), lambda: ctx.token_logprobs(x, [1, 2, 3], 1, 65), lambda: ctx.token_logprobs(x[:1], None, 1, 100)):
+        with pytest.raises(mlamoe.MMError) as e:
+            call()
+        assert e.value.status == -1

@@ -563,3 +563,20 @@ def test_many_rows_in_groups(monkeypatch, NH, B, QKN, VHD):
     monkeypatch.setenv("MLAMOE_MLA_PART_MAX", str(9 << 20))
     assert np.array_equal(a, prefix_case(NH, B, 210, 50, lens, QKN, VHD, seed=500 + NH))
     assert np.array_equal(w, window_case(NH, 2, B // 2, 400, 5, 90, [400, 311], QKN, VHD, seed=501 + NH))
+
+
+@pytest.mark.gpu
+def test_host_forms_refuse_arrays_too_short():
+    """Lengths, rows and heads that the kernels would read past."""
+    ctx, _ = loaded(16)
+    q, pre, c = np.zeros((3, 16, 192), np.float32), np.zeros((5, 576), np.uint16), np.zeros((3, 8, 576), np.uint16)
+    with ctx:
+        for call in (lambda: ctx.mla_prefix_decode(0, q, pre, c, [1, 2]), lambda: ctx.mla_prefix_decode(0, q, pre, c[:2]),
+                     lambda: ctx.mla_prefix_decode(0, q[:, :15], pre, c), lambda: ctx.mla_prefix_decode(0, q[..., :128], pre, c),
+                     lambda: ctx.mla_prefix_decode(0, q, pre[:, :512], c), lambda: ctx.mla_prefix_decode(0, q, pre, c[..., :512]),
+                     lambda: ctx.mla_window_decode(0, q[:, None], c[:2], 0, 4), lambda: ctx.mla_window_decode(0, q[:, None], c, 0, 4, [1]),
+                     lambda: ctx.mla_window_decode(0, q, c, 0, 4), lambda: ctx.mla_window_decode(0, q[:, None, :8], c, 0, 4),
+                     lambda: ctx.mla_window_decode(0, q[:, None], c[..., :512], 0, 4)):
+            with pytest.raises(mlamoe.MMError) as e:
+                call()
+            assert e.value.status == -1
