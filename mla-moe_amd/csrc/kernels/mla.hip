@@ -240,13 +240,13 @@ extern "C" __global__ __launch_bounds__(256) void mm_mla_wprep(mm_mla_wprep_args
         a.wukT[i] = a.kv_b[(h * (a.QKN + a.VHD) + d) * KVL + r];
     }
     const int ncol = (a.VHD + 15) / 16;
-    const size_t nf = (size_t)a.NH * ncol * MM_MLA_UVF_TILE;
+    const size_t nf = (size_t)a.NH * ncol * (MM_MLA_UVF_TILE / 8);   /* a lane's 8 latents at a time */
     for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < nf;
          i += (size_t)gridDim.x * blockDim.x) {
-        const int e = (int)(i % MM_MLA_UVF_TILE), l = e >> 3 & 63, r = 32 * (e >> 9) + 8 * (l >> 4) + (e & 7);
-        const size_t c = i / MM_MLA_UVF_TILE, h = c / ncol;
+        const int e = (int)(i % (MM_MLA_UVF_TILE / 8)), l = e & 63, r = 32 * (e >> 6) + 8 * (l >> 4);
+        const size_t c = i / (MM_MLA_UVF_TILE / 8), h = c / ncol;
         const size_t v = min((int)(c % ncol) * 16 + (l & 15), a.VHD - 1);
-        a.wuvf[i] = a.kv_b[(h * (a.QKN + a.VHD) + a.QKN + v) * KVL + r];
+        *(i32x4 *)(a.wuvf + 8 * i) = *(const i32x4 *)(a.kv_b + (h * (a.QKN + a.VHD) + a.QKN + v) * KVL + r);
     }
 }
 
