@@ -17,7 +17,8 @@
  * an element must beat.  A wave meets few such elements after its first chunk,
  * which starts from the n_top-th of the lanes' maxima.  All of this is written
  * once per kernel, in loops: unrolled over a chunk's elements it was instructions
- * to fetch (one row, 20 alternatives: 13 + 7 us; without any 4 + 2). */
+ * to fetch (one row, 20 alternatives: 13 + 7 us, in loops 9 + 5; without any 4 +
+ * 2, so that the selection still is most of a short call). */
 #define LP_VPL 16                  /* elements per lane and chunk */
 #define LP_CHUNK (LP_VPL * MM_WAVE)
 #define LP_WAVES 4

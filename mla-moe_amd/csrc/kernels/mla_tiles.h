@@ -22,8 +22,8 @@
  * rows of 16 heads over 4,096 keys).
  *
  * The matrix cores bound it: 2,176 cycles of products a tile on each of four
- * SIMDs on average, 64 rows of 16 heads over 32,768 keys 130 us in all, 1.12
- * PFLOP/s of pair products (a library's product of 8,192^3: 1.21).
+ * SIMDs on average, 64 rows of 16 heads over 32,768 keys 132 to 140 us in all, 1.05
+ * to 1.11 PFLOP/s of pair products (a library's product of 8,192^3: 1.21).
  *
  * LDS, per tile of 32 keys: latents 0..287 (576 bytes a row, four tiles of
  * them), 288..511 (448 bytes, three), k_pe (128 bytes, two): a part lives until
