@@ -88,20 +88,19 @@ __device__ __forceinline__ void tl_scores(const i32x4 (&qh)[18], const i32x4 (&q
  * in whatever order. */
 __device__ __forceinline__ uint32_t tl_not_finite(uint32_t r0, uint32_t r1, uint32_t kp) {
     const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5;
-    uint32_t top = 0;
+    uint32_t any = 0;
     auto look = [&](uint32_t p, int n) {
 #pragma unroll 1
         for (int i = 0; i < n; i++) {
             const i32x4 x = *(lds_w4)(uintptr_t)(p + 16 * i);
-            /* two bf16 each: an exponent of ones carries into the sign's place */
 #pragma unroll
-            for (int k = 0; k < 4; k++) top |= ((uint32_t)x[k] & 0x7f807f80u) + 0x00800080u;
+            for (int k = 0; k < 4; k++) any |= nonfinite2((uint32_t)x[k]);
         }
     };
     look(r0 + (uint32_t)(row * 576 + half * 288), 18);
     look(r1 + (uint32_t)(row * 448 + half * 224), 14);
     look(kp + (uint32_t)(row * 128 + half * 64), 4);
-    const uint64_t m = __builtin_amdgcn_ballot_w64((top & 0x80008000u) != 0);
+    const uint64_t m = __builtin_amdgcn_ballot_w64(any != 0);
     return (uint32_t)m | (uint32_t)(m >> 32);
 }
 
